@@ -314,6 +314,95 @@ int per_update_priorities_shard_count(const per_store_t* store, int64_t base, co
                                       const float* td, int64_t n, const int64_t* count,
                                       void* stream);
 
+/* ---- operators of the learner that trains on the sampled batches (no
+ * counterpart in the reference's library; its learner,
+ * experiments/sac.py, takes them from PyTorch). A step runs them between
+ * sample and update_priorities: layer norm in the networks, forward and
+ * backward, then the clipping of all gradients by their global norm. */
+
+/* element types */
+#define PER_F32 0
+#define PER_BF16 1
+#define PER_F16 2
+
+/* Layer norm of `rows` rows of `dim` values. Arithmetic is float32 whatever
+ * the types; a 16-bit result is rounded once. */
+typedef struct per_norm {
+  int64_t rows;         /* >= 0 */
+  int64_t dim;          /* 1 .. 2^31 - 1 */
+  int32_t dtype;        /* PER_* type of x, y, dy, dx */
+  int32_t param_dtype;  /* PER_* type of weight, bias and their gradients: PER_F32 or `dtype` */
+  float eps;            /* >= 0, added to the variance (forward only) */
+} per_norm_t;
+
+/* y[r][c] = (x[r][c] - m_r) * rstd_r * weight[c] + bias[c], with m_r the mean
+ * of row r and rstd_r = 1 / sqrt(var_r + eps), var_r the mean squared
+ * distance from m_r. Strides are in elements between the starts of rows
+ * (>= dim), any alignment of the element size. weight and / or bias may be
+ * NULL (1 and 0). mean (float64[rows]) and rstd (float32[rows]) receive the
+ * rows' statistics for per_layer_norm_backward(); pass NULL for both when no
+ * backward pass follows. y must not overlap x. */
+int per_layer_norm(const per_norm_t* norm, const void* x, int64_t x_stride, const void* weight,
+                   const void* bias, void* y, int64_t y_stride, double* mean, float* rstd,
+                   void* stream);
+
+/* Bytes of `workspace` (16-byte aligned) that per_layer_norm_backward() needs
+ * on the current device for this norm; -1 for a bad descriptor. */
+int64_t per_layer_norm_backward_workspace(const per_norm_t* norm);
+
+/* Gradients of per_layer_norm() from dy: with g = dy * weight and
+ * h = (x - mean) * rstd, dx = rstd * (g - avg(g) - h * avg(g * h)) row by row,
+ * dweight = sum over rows of dy * h, dbias = sum over rows of dy. Any of dx,
+ * dweight, dbias may be NULL (not wanted); weight is NULL where the forward
+ * pass had none. dy_stride may be 0 (one row for all). Sums over rows are
+ * float32 in a fixed order: the same call on the same kind of GPU gives the
+ * same bits. With rows == 0, dweight and dbias are zeroed. The workspace is
+ * scratch for the duration of the call's work: calls that may overlap on the
+ * GPU need one each. Outputs must not overlap inputs. */
+int per_layer_norm_backward(const per_norm_t* norm, const void* dy, int64_t dy_stride,
+                            const void* x, int64_t x_stride, const void* weight,
+                            const double* mean, const float* rstd, void* dx, int64_t dx_stride,
+                            void* dweight, void* dbias, void* workspace, int64_t workspace_bytes,
+                            void* stream);
+
+/* One tensor of a list: `count` values of one type, dense in memory, in any
+ * order (a norm does not depend on it). */
+typedef struct per_tensor {
+  void* data;     /* aligned to the element size; may be NULL when count is 0 */
+  int64_t count;
+  int32_t dtype;  /* PER_* type */
+  int32_t reserved;
+} per_tensor_t;
+
+/* norms over a list of tensors */
+#define PER_NORM_L1 1
+#define PER_NORM_L2 2
+#define PER_NORM_INF 3
+
+/* Bytes of `workspace` (16-byte aligned) that a norm of `n` tensors needs. */
+int64_t per_grad_norm_workspace(int64_t n);
+
+/* *norm = the norm of all values of all tensors (float32 on the device): the
+ * root of the sum of squares, the sum of absolute values, or the largest one.
+ * NaN where a value is NaN. Values whose squares leave the float32 range are
+ * summed in float64. `tensors` is a host array, read during the call only.
+ * Workspace as in per_layer_norm_backward(). */
+int per_grad_norm(const per_tensor_t* tensors, int64_t n, int32_t kind, float* norm,
+                  void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Multiply every value by min(1, max_norm / (*norm + 1e-6)), in float32 and
+ * rounded once; tensors are not touched where that factor is 1. `norm` is a
+ * device float32 (of per_grad_norm(), or joined over the ranks of a job). The
+ * factor is NaN where *norm is NaN, and 0 where it is infinite. No two tensors
+ * may overlap. */
+int per_scale_grads(const per_tensor_t* tensors, int64_t n, float max_norm, const float* norm,
+                    void* stream);
+
+/* per_grad_norm() and per_scale_grads() in one call: the clipping of the
+ * gradients by their global norm. *norm is the norm before the clipping. */
+int per_clip_grad_norm(const per_tensor_t* tensors, int64_t n, int32_t kind, float max_norm,
+                       float* norm, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Human-readable name of a PER_* return code. */
 const char* per_error_string(int code);
 

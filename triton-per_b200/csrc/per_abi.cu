@@ -9,17 +9,7 @@
 #include "per_b200.h"
 #include "per_internal.h"
 
-#include <nvtx3/nvToolsExt.h>
-
 namespace {
-
-// NVTX range around an entry point (profilers show each call; without a
-// profiler attached this is a few tens of nanoseconds)
-struct PerRange {
-  explicit PerRange(const char* name) { nvtxRangePushA(name); }
-  ~PerRange() { nvtxRangePop(); }
-};
-
 
 thread_local int g_last_cuda = 0;
 

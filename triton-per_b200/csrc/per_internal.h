@@ -2,9 +2,17 @@
 #pragma once
 
 #include <cuda_runtime.h>
+#include <nvtx3/nvToolsExt.h>
 #include <stdint.h>
 
 #include "per_common.cuh"
+
+// NVTX range around an entry point (profilers show each call; without a
+// profiler attached this is a few tens of nanoseconds)
+struct PerRange {
+  explicit PerRange(const char* name) { nvtxRangePushA(name); }
+  ~PerRange() { nvtxRangePop(); }
+};
 
 // Record a CUDA error for per_last_cuda_error() and return PER_ERR_CUDA.
 int per_record_cuda(cudaError_t e);
@@ -71,3 +79,22 @@ int per_launch_sample_sharded_p2p(const PerTree& t, int32_t rank, int32_t world,
                                   cudaStream_t stream);
 int per_launch_normalize(float* w, const int64_t* count, const float* gmax, int64_t cap,
                          cudaStream_t stream);
+
+// Operators of the learner. Arguments are checked by the entry points; NULL
+// pointers mean "absent" as described in per_b200.h.
+int per_launch_layer_norm(const per_norm_t& n, const void* x, int64_t x_stride, const void* weight,
+                          const void* bias, void* y, int64_t y_stride, double* mean, float* rstd,
+                          cudaStream_t stream);
+int64_t per_layer_norm_backward_bytes(const per_norm_t& n);
+int per_launch_layer_norm_backward(const per_norm_t& n, const void* dy, int64_t dy_stride,
+                                   const void* x, int64_t x_stride, const void* weight,
+                                   const double* mean, const float* rstd, void* dx,
+                                   int64_t dx_stride, void* dweight, void* dbias, void* workspace,
+                                   cudaStream_t stream);
+int64_t per_grad_norm_bytes(int64_t n);
+int per_launch_grad_norm(const per_tensor_t* tensors, int64_t n, int32_t kind, float* norm,
+                         void* workspace, cudaStream_t stream);
+int per_launch_scale_grads(const per_tensor_t* tensors, int64_t n, float max_norm,
+                           const float* norm, cudaStream_t stream);
+int per_launch_clip_grad_norm(const per_tensor_t* tensors, int64_t n, int32_t kind, float max_norm,
+                              float* norm, void* workspace, cudaStream_t stream);

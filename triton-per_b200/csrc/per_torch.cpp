@@ -168,8 +168,11 @@ class Engine {
 
 }  // namespace
 
+void per_register_learner(py::module_& m);  // per_torch_learner.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
-  m.doc() = "torch-tensor binding of the per_b200 sample / update calls";
+  m.doc() = "torch-tensor binding of the per_b200 sample / update calls and learner operators";
+  per_register_learner(m);
   py::class_<Engine>(m, "Engine")
       .def(py::init<int64_t, int64_t, std::vector<std::string>, std::vector<int64_t>, int64_t,
                     int64_t>())

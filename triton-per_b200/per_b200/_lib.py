@@ -85,6 +85,25 @@ class Field(ctypes.Structure):
     ]
 
 
+class Norm(ctypes.Structure):
+    _fields_ = [
+        ("rows", i64),
+        ("dim", i64),
+        ("dtype", i32),
+        ("param_dtype", i32),
+        ("eps", ctypes.c_float),
+    ]
+
+
+class Tensor(ctypes.Structure):
+    _fields_ = [
+        ("data", vp),
+        ("count", i64),
+        ("dtype", i32),
+        ("reserved", i32),
+    ]
+
+
 # name -> (restype, argtypes); every function declared in include/per_b200.h
 SIGNATURES = {
     "per_layout": (ctypes.c_int, [i64, ctypes.POINTER(Layout)]),
@@ -118,6 +137,15 @@ SIGNATURES = {
     "per_update_priorities_shard": (ctypes.c_int, [ctypes.POINTER(Store), i64, vp, vp, i64, vp]),
     "per_update_priorities_shard_count": (ctypes.c_int, [ctypes.POINTER(Store), i64, vp, vp, i64, vp,
                                                          vp]),
+    "per_layer_norm": (ctypes.c_int, [ctypes.POINTER(Norm), vp, i64, vp, vp, vp, i64, vp, vp, vp]),
+    "per_layer_norm_backward_workspace": (i64, [ctypes.POINTER(Norm)]),
+    "per_layer_norm_backward": (ctypes.c_int, [ctypes.POINTER(Norm), vp, i64, vp, i64, vp, vp, vp, vp,
+                                               i64, vp, vp, vp, i64, vp]),
+    "per_grad_norm_workspace": (i64, [i64]),
+    "per_grad_norm": (ctypes.c_int, [ctypes.POINTER(Tensor), i64, i32, vp, vp, i64, vp]),
+    "per_scale_grads": (ctypes.c_int, [ctypes.POINTER(Tensor), i64, ctypes.c_float, vp, vp]),
+    "per_clip_grad_norm": (ctypes.c_int, [ctypes.POINTER(Tensor), i64, i32, ctypes.c_float, vp, vp,
+                                          i64, vp]),
     "per_error_string": (ctypes.c_char_p, [ctypes.c_int]),
     "per_last_cuda_error": (ctypes.c_int, []),
     "per_abi_version": (ctypes.c_int, []),

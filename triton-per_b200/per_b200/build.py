@@ -66,9 +66,9 @@ def build(force: bool = False, verbose: bool = False) -> str:
     return LIB
 
 
-# ---- the torch-tensor binding (csrc/per_torch.cpp -> per_b200/_per_torch*.so):
+# ---- the torch-tensor binding (csrc/per_torch*.cpp -> per_b200/_per_torch*.so):
 # a C++ extension linked against libper_b200.so (found next to it at run time)
-BINDING_SRC = os.path.join(CSRC, "per_torch.cpp")
+BINDING_SRCS = [os.path.join(CSRC, f) for f in ("per_torch.cpp", "per_torch_learner.cpp")]
 
 
 def binding_path() -> str:
@@ -84,7 +84,7 @@ def build_binding(force: bool = False, verbose: bool = False) -> str:
     import torch.utils.cpp_extension as ext
 
     out = binding_path()
-    deps = [BINDING_SRC, LIB, os.path.join(INCLUDE, "per_b200.h")]
+    deps = [*BINDING_SRCS, LIB, os.path.join(INCLUDE, "per_b200.h")]
     if not force and os.path.exists(out) and all(os.path.getmtime(d) <= os.path.getmtime(out)
                                                  for d in deps):
         return out
@@ -98,7 +98,7 @@ def build_binding(force: bool = False, verbose: bool = False) -> str:
     cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-w",
            f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_EXTENSION_NAME=_per_torch",
            "-DTORCH_API_INCLUDE_EXTENSION_H",
-           *[f"-I{i}" for i in incs], BINDING_SRC, "-o", out + ".tmp",
+           *[f"-I{i}" for i in incs], *BINDING_SRCS, "-o", out + ".tmp",
            f"-L{libdir}", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda",
            "-ltorch_python", f"-Wl,-rpath,{libdir}",
            f"-L{PKG}", "-lper_b200", "-Wl,-rpath,$ORIGIN"]

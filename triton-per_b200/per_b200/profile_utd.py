@@ -1,13 +1,16 @@
 """Replay share of a high-UTD training step on the B200 engine.
 
     python -m per_b200.profile_utd --utd 32 --batch-size 256 --steps 60 [--num-q 10] [--trace out.json]
+                                   [--layer-norm] [--max-grad-norm 10]
 
 The caller context of the hot path (the reference measures it with
 bench/profile_utd.py:76-97): a SAC-style update phase — an MLP actor and
 `num_q` MLP critics (two hidden layers of 256), Adam — where every gradient
 step samples a prioritized batch, computes TD errors and writes them back as
 priorities, `utd` times per environment step, with one new transition added
-per environment step. It reports the fraction of step time spent in the
+per environment step. `--layer-norm` puts a layer norm behind every hidden
+layer and `--max-grad-norm` clips the gradients' global norm, as learners at
+such ratios commonly do, both on this engine's kernels (per_b200.learner). It reports the fraction of step time spent in the
 replay calls (sample + update_priorities).
 
 Unlike a host timer around synchronised calls, each phase is bracketed by
@@ -33,20 +36,26 @@ import torch
 import torch.nn as nn
 
 from .buffer import PERBuffer
+from .learner import LayerNorm, clip_grad_norm_
 
 
-def mlp(i: int, o: int, h: int = 256) -> nn.Module:
-    return nn.Sequential(nn.Linear(i, h), nn.ReLU(), nn.Linear(h, h), nn.ReLU(), nn.Linear(h, o))
+def mlp(i: int, o: int, h: int = 256, layer_norm: bool = False) -> nn.Module:
+    norm = (lambda: [LayerNorm(h)]) if layer_norm else (lambda: [])
+    return nn.Sequential(nn.Linear(i, h), *norm(), nn.ReLU(), nn.Linear(h, h), *norm(), nn.ReLU(),
+                         nn.Linear(h, o))
 
 
 class Learner:
     """Actor + critics with one optimiser; step() returns |TD| per sample."""
 
-    def __init__(self, obs_dim: int, act_dim: int, num_q: int, device):
-        self.actor = mlp(obs_dim, act_dim).to(device)
-        self.qs = nn.ModuleList([mlp(obs_dim + act_dim, 1) for _ in range(num_q)]).to(device)
-        self.opt = torch.optim.Adam(list(self.actor.parameters()) + list(self.qs.parameters()),
-                                    lr=3e-4)
+    def __init__(self, obs_dim: int, act_dim: int, num_q: int, device, layer_norm: bool = False,
+                 max_grad_norm: float | None = None):
+        self.actor = mlp(obs_dim, act_dim, layer_norm=layer_norm).to(device)
+        self.qs = nn.ModuleList([mlp(obs_dim + act_dim, 1, layer_norm=layer_norm)
+                                 for _ in range(num_q)]).to(device)
+        self.params = list(self.actor.parameters()) + list(self.qs.parameters())
+        self.opt = torch.optim.Adam(self.params, lr=3e-4)
+        self.max_grad_norm = max_grad_norm
 
     def step(self, batch: dict, w: torch.Tensor) -> torch.Tensor:
         obs, act, rew = batch["obs"], batch["action"], batch["reward"].squeeze(-1)
@@ -55,6 +64,8 @@ class Learner:
         loss = sum((w * td.pow(2)).mean() for td in tds) + 1e-3 * self.actor(obs).pow(2).mean()
         self.opt.zero_grad(set_to_none=True)
         loss.backward()
+        if self.max_grad_norm is not None:
+            clip_grad_norm_(self.params, self.max_grad_norm)
         self.opt.step()
         return tds[0].detach().abs()
 
@@ -62,11 +73,12 @@ class Learner:
 def run(utd: int = 32, batch_size: int = 256, capacity: int = 1_000_000, obs_dim: int = 32,
         act_dim: int = 8, num_q: int = 2, steps: int = 60, warmup: int = 10, fill: int = 200_000,
         device: str = "cuda", trace: str | None = None, seed: int = 0, buffer=None,
-        timing: str = "events") -> dict:
+        timing: str = "events", layer_norm: bool = False,
+        max_grad_norm: float | None = None) -> dict:
     """buffer: a buffer with the PERBuffer API built for these fields and
     capacity (default: this engine's PERBuffer). timing "events": CUDA events
     on the stream, nothing synchronised; "wall": host clock around
-    synchronised phases."""
+    synchronised phases. layer_norm, max_grad_norm: the learner's (see Learner)."""
     if timing not in ("events", "wall"):
         raise ValueError(f"timing must be 'events' or 'wall', not {timing!r}")
     torch.manual_seed(seed)
@@ -75,7 +87,7 @@ def run(utd: int = 32, batch_size: int = 256, capacity: int = 1_000_000, obs_dim
     buf = buffer if buffer is not None else PERBuffer(capacity, fields, device=dev)
     n = min(capacity, fill)
     buf.add({k: torch.randn(n, d, device=dev) for k, d in fields.items()})
-    learner = Learner(obs_dim, act_dim, num_q, dev)
+    learner = Learner(obs_dim, act_dim, num_q, dev, layer_norm, max_grad_norm)
     new_row = {k: torch.randn(1, d, device=dev) for k, d in fields.items()}
 
     stream = torch.cuda.current_stream(dev)
@@ -137,6 +149,7 @@ def run(utd: int = 32, batch_size: int = 256, capacity: int = 1_000_000, obs_dim
     elapsed = total.elapsed_time(end)
     result = {
         "utd": utd, "batch_size": batch_size, "capacity": capacity, "num_q": num_q,
+        "layer_norm": layer_norm, "max_grad_norm": max_grad_norm,
         "steps": steps, "timing": timing, "replay_ms": replay, "learn_ms": learn,
         "step_ms": elapsed / steps,
         "replay_share": replay / (replay + learn) if replay + learn > 0 else 0.0,
@@ -170,10 +183,15 @@ def main() -> None:
     ap.add_argument("--device", default="cuda")
     ap.add_argument("--trace", default=None, help="Chrome trace output path")
     ap.add_argument("--timing", default="events", choices=["events", "wall"])
+    ap.add_argument("--layer-norm", action="store_true",
+                    help="a layer norm behind every hidden layer")
+    ap.add_argument("--max-grad-norm", type=float, default=None,
+                    help="clip the gradients' global norm")
     args = ap.parse_args()
     print(json.dumps(run(args.utd, args.batch_size, args.capacity, args.obs_dim, args.act_dim,
                          args.num_q, args.steps, args.warmup, device=args.device,
-                         trace=args.trace, timing=args.timing)))
+                         trace=args.trace, timing=args.timing, layer_norm=args.layer_norm,
+                         max_grad_norm=args.max_grad_norm)))
 
 
 if __name__ == "__main__":
