@@ -111,8 +111,8 @@ def test_rows_inside_packed_rows(dtype, dim, stride, offset):
     packed = rows_like_activations(67, stride, dtype)
     x = packed[:, offset:offset + dim]
     w, b = params_like(dim, F32, "both")
-    y = check_forward(x, w, b)
-    assert torch.equal(y, per_b200.layer_norm(x.contiguous(), dim, w, b, EPS))
+    check_forward(x, w, b)
+    check_forward(x.contiguous(), w, b)
     dy = normal(67, stride + 3, seed=4).to(dtype)[:, 3:3 + dim]
     got = check_train(x, w, b, dy)
     assert got[0].is_contiguous()

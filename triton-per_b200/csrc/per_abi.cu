@@ -20,7 +20,7 @@ struct OccEntry {
   size_t smem;
   int ctas;
 };
-constexpr int kOccSlots = 256;
+constexpr int kOccSlots = 1024;
 OccEntry g_occ[kOccSlots];
 int g_occ_n = 0;
 std::mutex g_occ_mu;
@@ -163,7 +163,7 @@ int per_set_smem(const void* fn, size_t smem) {
     int device;
     const void* fn;
     size_t smem;
-  } done[64];
+  } done[512];
   static int n_done = 0;
   std::lock_guard<std::mutex> lk(mu);
   for (int i = 0; i < n_done; ++i)
@@ -179,7 +179,7 @@ int per_set_smem(const void* fn, size_t smem) {
       done[i].smem = smem;
       return PER_OK;
     }
-  if (n_done < 64) done[n_done++] = {dev, fn, smem};
+  if (n_done < 512) done[n_done++] = {dev, fn, smem};
   return PER_OK;
 }
 
@@ -208,6 +208,28 @@ cudaError_t per_launch(const void* fn, unsigned grid, unsigned threads, size_t s
   }
   cfg.attrs = attr;
   cfg.numAttrs = (coop || pdl_enabled()) ? 1 : 0;
+  cudaError_t e = cudaLaunchKernelExC(&cfg, fn, args);
+  if (e != cudaSuccess) return e;
+  return cudaGetLastError();
+}
+
+cudaError_t per_launch_cluster(const void* fn, unsigned grid, unsigned threads, size_t smem,
+                               unsigned cluster, cudaStream_t stream, void** args) {
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
   cudaError_t e = cudaLaunchKernelExC(&cfg, fn, args);
   if (e != cudaSuccess) return e;
   return cudaGetLastError();

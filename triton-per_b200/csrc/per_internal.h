@@ -41,6 +41,10 @@ int per_set_smem(const void* fn, size_t smem);
 cudaError_t per_launch(const void* fn, unsigned grid, unsigned threads, size_t smem,
                        cudaStream_t stream, void** args, bool grid_sync);
 
+// Launch `fn` in clusters of `cluster` CTAs (grid a multiple of it).
+cudaError_t per_launch_cluster(const void* fn, unsigned grid, unsigned threads, size_t smem,
+                               unsigned cluster, cudaStream_t stream, void** args);
+
 // In-kernel uniforms: Philox4x32-10 stream `seed`, position in *counter
 // (device), advanced by the kernel by the batch size.
 struct PerRng {

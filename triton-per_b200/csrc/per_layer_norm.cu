@@ -67,6 +67,468 @@ __device__ __forceinline__ float2 block_sum2(float a, float b) {
   return make_float2(warp_sum(v.x), warp_sum(v.y));
 }
 
+// VEC values that are loaded and stored at once.
+template <typename T, int VEC>
+struct alignas(VEC * sizeof(T)) Pack {
+  T v[VEC];
+};
+
+template <typename T, int VEC>
+__device__ __forceinline__ Pack<T, VEC> load(const T* p) {
+  Pack<T, VEC> r;
+  if constexpr (VEC * sizeof(T) == 32) {
+    const uint4 a = reinterpret_cast<const uint4*>(p)[0], b = reinterpret_cast<const uint4*>(p)[1];
+    reinterpret_cast<uint4*>(&r)[0] = a;
+    reinterpret_cast<uint4*>(&r)[1] = b;
+  } else if constexpr (VEC * sizeof(T) == 16) {
+    *reinterpret_cast<uint4*>(&r) = *reinterpret_cast<const uint4*>(p);
+  } else {
+    static_assert(VEC == 1, "single values, or 16 and 32 bytes");
+    r.v[0] = p[0];
+  }
+  return r;
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void store(T* p, const Pack<T, VEC>& r) {
+  if constexpr (VEC == 1)
+    p[0] = r.v[0];
+  else
+    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(&r);
+}
+
+// The threads of a row: LANES of them (a power of two, several rows per
+// warp), a whole CTA (LANES 0), or a cluster of CTAs (LANES -1, rows too long
+// for one). Thread `lane` of `width` holds the vectors lane, lane + width, ...
+// of VEC values, NV of them at most.
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+
+template <int LANES>
+struct Row {
+  int lane, width;     // of this thread in its row
+  int64_t base, step;  // first row of this warp, rows between two of its turns
+  int mine;            // this thread's row is base + mine
+  __device__ __forceinline__ Row() {
+    if constexpr (LANES > 0) {
+      const int per_cta = blockDim.x / LANES;
+      lane = threadIdx.x % LANES;
+      width = LANES;
+      base = (int64_t)blockIdx.x * per_cta + (threadIdx.x & ~31) / LANES;
+      step = (int64_t)gridDim.x * per_cta;
+      mine = (threadIdx.x & 31) / LANES;
+    } else {
+      const int ctas = LANES == 0 ? 1 : (int)cluster_size();
+      lane = threadIdx.x + (LANES == 0 ? 0 : (int)(cluster_rank() * blockDim.x));
+      width = blockDim.x * ctas;
+      base = blockIdx.x / ctas;
+      step = gridDim.x / ctas;
+      mine = 0;
+    }
+  }
+};
+
+template <int LANES>
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+  for (int o = (LANES > 0 ? LANES : 32) / 2; o; o >>= 1) v += __shfl_xor_sync(PER_FULL_MASK, v, o);
+  return v;
+}
+
+// What the warps of a row hand to one another: each warp's words go to every
+// CTA of the row, then one barrier. Two buffers by turns, so that one barrier
+// per exchange is enough: a buffer is written again only after the barrier of
+// the next exchange, which follows every read of it.
+constexpr int kMaxCluster = 8;
+template <int LANES>
+struct Exchange {
+  float3 slot[2][LANES == 0 ? 32 : 32 * kMaxCluster];
+};
+
+template <int LANES>
+__device__ __forceinline__ void put(Exchange<LANES>& e, int turn, float3 v) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if constexpr (LANES == 0) {
+    if (lane == 0) e.slot[turn][warp] = v;
+    __syncthreads();
+  } else {
+    const int ctas = (int)cluster_size();
+    if (lane < ctas) {  // lane = the CTA that the warp's words go to
+      const float3* at = &e.slot[turn][cluster_rank() * (blockDim.x >> 5) + warp];
+      const uint32_t local = (uint32_t)__cvta_generic_to_shared(at);
+      uint32_t remote;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(lane));
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(v.x) : "memory");
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote + 4), "f"(v.y) : "memory");
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote + 8), "f"(v.z) : "memory");
+    }
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+}
+
+// Sums of a and b over the threads of a row.
+template <int LANES>
+__device__ __forceinline__ float2 row_sum2(float a, float b, Exchange<LANES>& e, int& turn) {
+  a = lanes_sum<LANES>(a);
+  b = lanes_sum<LANES>(b);
+  if constexpr (LANES > 0) {
+    return make_float2(a, b);
+  } else {
+    const int warps = (blockDim.x >> 5) * (LANES == 0 ? 1 : (int)cluster_size());
+    put<LANES>(e, turn, make_float3(a, b, 0.f));
+    a = b = 0.f;
+    for (int q = threadIdx.x & 31; q < warps; q += 32) {
+      a += e.slot[turn][q].x;
+      b += e.slot[turn][q].y;
+    }
+    turn ^= 1;
+    return make_float2(lanes_sum<0>(a), lanes_sum<0>(b));
+  }
+}
+
+// A thread's own copies on their way into shared memory, STAGES rows ahead:
+// it waits for and reads only what it has copied itself, so no barrier is
+// needed. 16-byte vectors go by cp.async; single values are fetched into
+// registers one row ahead.
+template <typename T, int VEC, int NV, int STAGES>
+struct Ring {
+  static constexpr bool kAsync = VEC * sizeof(T) == 16;
+  static constexpr int kStages = kAsync ? STAGES : 1;
+  static constexpr size_t kBytes = kAsync ? STAGES * NV * 16 : 0;  // per thread
+  uint32_t at;
+  Pack<T, VEC> reg[kAsync ? 1 : NV];
+
+  __device__ __forceinline__ explicit Ring(const void* smem) {
+    at = (uint32_t)__cvta_generic_to_shared(smem) + threadIdx.x * 16;
+  }
+  __device__ __forceinline__ void fetch(int stage, int k, const T* p, bool in) {
+    if (!in) return;
+    if constexpr (kAsync)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                       at + (stage * NV + k) * blockDim.x * 16),
+                   "l"(p)
+                   : "memory");
+    else
+      reg[k] = load<T, VEC>(p);
+  }
+  static __device__ __forceinline__ void commit() {
+    if constexpr (kAsync) asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  // the oldest stage has landed (one group per stage is in flight)
+  static __device__ __forceinline__ void wait() {
+    if constexpr (kAsync) asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+  }
+  __device__ __forceinline__ Pack<T, VEC> get(int stage, int k) {
+    if constexpr (kAsync) {
+      uint4 u;
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+                   : "r"(at + (stage * NV + k) * blockDim.x * 16)
+                   : "memory");
+      Pack<T, VEC> r;
+      *reinterpret_cast<uint4*>(&r) = u;
+      return r;
+    } else {
+      return reg[k];
+    }
+  }
+};
+
+// Threads of a CTA that holds a row: 1024, or half of it for single values,
+// whose columns cost a thread more registers than 64.
+constexpr int row_threads(int vec) { return vec == 1 ? 512 : 1024; }
+
+// Before a CTA writes into another one's shared memory, that one has to run.
+template <int LANES>
+__device__ __forceinline__ void cluster_begins() {
+  if constexpr (LANES < 0) {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+}
+
+constexpr int kFwdStages = 4;
+constexpr int kBwdStages = 3;
+
+// ---- forward, rows in registers
+template <typename T, typename P, int VEC, int NV, int LANES>
+__global__ void __launch_bounds__(LANES > 0 ? 128 : row_threads(VEC)) per_layer_norm_kernel(const Fwd f) {
+  __shared__ Exchange<LANES> ex;
+  extern __shared__ __align__(16) unsigned char dyn[];
+  const Row<LANES> t;
+  using R = Ring<T, VEC, NV, kFwdStages>;
+  R ring(dyn);
+  int turn = 0, stage = 0;
+  const float n = (float)f.dim;
+  const T* x = static_cast<const T*>(f.x);
+  T* y = static_cast<T*>(f.y);
+  int count = 0;  // values of this warp (of a row that spans warps)
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = (t.lane + k * t.width) * VEC;
+    count += c < f.dim ? VEC : 0;
+  }
+  if constexpr (LANES <= 0) count = __reduce_add_sync(PER_FULL_MASK, count);
+  cluster_begins<LANES>();
+  per_wait_previous_grid();
+  auto fetch = [&](int st, int64_t row) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (t.lane + k * t.width) * VEC;
+      ring.fetch(st, k, x + row * f.x_stride + c, row < f.rows && c < f.dim);
+    }
+    R::commit();
+  };
+#pragma unroll
+  for (int k = 0; k < R::kStages; ++k) fetch(k, t.base + t.mine + k * t.step);
+  Pack<P, VEC> w[NV], b[NV];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = (t.lane + k * t.width) * VEC;
+    if (c < f.dim && f.w) w[k] = load<P, VEC>(static_cast<const P*>(f.w) + c);
+    if (c < f.dim && f.b) b[k] = load<P, VEC>(static_cast<const P*>(f.b) + c);
+  }
+  for (int64_t base = t.base; base < f.rows; base += t.step) {
+    const int64_t row = base + t.mine;
+    float v[NV][VEC];
+    float a = 0.f;
+    R::wait();
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const bool in = (t.lane + k * t.width) * VEC < f.dim;
+      const Pack<T, VEC> q = ring.get(stage, k);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        v[k][j] = in ? per_to_f32(q.v[j]) : 0.f;
+        a += v[k][j];
+      }
+    }
+    fetch(stage, row + R::kStages * t.step);
+    stage = stage + 1 == R::kStages ? 0 : stage + 1;
+    // distances from a first mean: the row's, or (rows that span warps) the warp's
+    const float own = LANES > 0 ? n : (float)count;
+    float s = lanes_sum<LANES>(a) / own;
+    if (LANES <= 0 && count == 0) s = 0.f;
+    float d1 = 0.f, d2 = 0.f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const bool in = (t.lane + k * t.width) * VEC < f.dim;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        v[k][j] = in ? v[k][j] - s : 0.f;
+        d1 += v[k][j];
+        d2 = fmaf(v[k][j], v[k][j], d2);
+      }
+    }
+    d1 = lanes_sum<LANES>(d1);
+    d2 = lanes_sum<LANES>(d2);
+    float shift, var;      // h = (v - shift) r
+    double mean;
+    if constexpr (LANES > 0) {
+      shift = d1 / n;
+      var = d2 / n - shift * shift;
+      mean = (double)s + (double)shift;
+    } else {
+      // Warp q of m_q values: mean s_q + d1_q / m_q, squares around it d2_q - d1_q^2 / m_q. Seen
+      // from s_0 its mean lies at z_q; the row's at z = sum m_q z_q / n, and the row's squares are
+      // the warps' plus m_q (z_q - z)^2 each.
+      const int warps = (blockDim.x >> 5) * (LANES == 0 ? 1 : (int)cluster_size());
+      const float m1 = count ? d1 / own : 0.f;
+      put<LANES>(ex, turn, make_float3(s, m1, fmaxf(d2 - d1 * m1, 0.f)));
+      const float s0 = ex.slot[turn][0].x;
+      constexpr int Q = LANES == 0 ? 1 : kMaxCluster;
+      float z = 0.f, sq = 0.f, zq[Q], mq[Q];
+#pragma unroll
+      for (int i = 0; i < Q; ++i) {
+        const int q = (threadIdx.x & 31) + 32 * i;
+        zq[i] = mq[i] = 0.f;
+        if (q >= warps) continue;
+        const float3 o = ex.slot[turn][q];
+        // values of warp q: its vectors q * 32 + l + k width below dim / VEC
+        int vecs = 0;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+          const int left = f.dim / VEC - q * 32 - k * t.width;
+          vecs += left < 0 ? 0 : left > 32 ? 32 : left;
+        }
+        mq[i] = (float)(vecs * VEC);
+        zq[i] = vecs ? (o.x - s0) + o.y : 0.f;
+        z = fmaf(mq[i], zq[i], z);
+        sq += o.z;
+      }
+      turn ^= 1;
+      z = lanes_sum<0>(z) / n;
+#pragma unroll
+      for (int i = 0; i < Q; ++i) sq = fmaf(mq[i] * (zq[i] - z), zq[i] - z, sq);
+      var = lanes_sum<0>(sq) / n;
+      shift = z - (s - s0);
+      mean = (double)s0 + (double)z;
+    }
+    const float r = rsqrtf(fmaxf(var, 0.f) + f.eps);
+    if (row < f.rows) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int c = (t.lane + k * t.width) * VEC;
+        if (c >= f.dim) continue;
+        Pack<T, VEC> o;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          float h = (v[k][j] - shift) * r;
+          if (f.w) h *= per_to_f32(w[k].v[j]);
+          if (f.b) h += per_to_f32(b[k].v[j]);
+          o.v[j] = per_from_f32<T>(h);
+        }
+        store<T, VEC>(y + row * f.y_stride + c, o);
+      }
+      if (f.mean && t.lane == 0) {
+        f.mean[row] = mean;
+        f.rstd[row] = r;
+      }
+    }
+  }
+}
+
+// ---- backward, rows in registers: dx, and the column sums of this CTA's
+// rows. Each thread keeps the sums of its columns while the CTA walks down
+// the rows; at the end the row groups of a CTA are joined in shared memory
+// and the CTA writes one partial row of dw and db.
+template <typename T, typename P, int VEC, int NV, int LANES>
+__global__ void __launch_bounds__(LANES > 0 ? 256 : row_threads(VEC)) per_layer_norm_backward_kernel(const Bwd g) {
+  __shared__ Exchange<LANES> ex;
+  extern __shared__ __align__(16) unsigned char dyn[];
+  const Row<LANES> t;
+  using R = Ring<T, VEC, 2 * NV, kBwdStages>;
+  R ring(dyn);
+  int turn = 0, stage = 0;
+  const float n = (float)g.dim;
+  const T* x = static_cast<const T*>(g.x);
+  const T* dy = static_cast<const T*>(g.dy);
+  T* dx = static_cast<T*>(g.dx);
+  cluster_begins<LANES>();
+  per_wait_previous_grid();
+  auto fetch = [&](int st, int64_t row) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (t.lane + k * t.width) * VEC;
+      ring.fetch(st, 2 * k, x + row * g.x_stride + c, row < g.rows && c < g.dim);
+      ring.fetch(st, 2 * k + 1, dy + row * g.dy_stride + c, row < g.rows && c < g.dim);
+    }
+    R::commit();
+  };
+  double nm = 0.0;
+  float nr = 0.f;
+  auto fetch_stats = [&](int64_t row) {
+    if (row >= g.rows) return;
+    nm = g.mean[row];
+    nr = g.rstd[row];
+  };
+#pragma unroll
+  for (int k = 0; k < R::kStages; ++k) fetch(k, t.base + t.mine + k * t.step);
+  fetch_stats(t.base + t.mine);
+  Pack<P, VEC> w[NV];
+  float aw[NV][VEC], ab[NV][VEC];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = (t.lane + k * t.width) * VEC;
+    if (c < g.dim && g.w) w[k] = load<P, VEC>(static_cast<const P*>(g.w) + c);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) aw[k][j] = ab[k][j] = 0.f;
+  }
+  for (int64_t base = t.base; base < g.rows; base += t.step) {
+    const int64_t row = base + t.mine;
+    const float hi = (float)nm, lo = (float)(nm - (double)hi), r = nr;
+    float h[NV][VEC], gv[NV][VEC];
+    float s1 = 0.f, s2 = 0.f;
+    R::wait();
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const bool in = row < g.rows && (t.lane + k * t.width) * VEC < g.dim;
+      const Pack<T, VEC> qx = ring.get(stage, 2 * k), qy = ring.get(stage, 2 * k + 1);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        h[k][j] = in ? (per_to_f32(qx.v[j]) - hi - lo) * r : 0.f;
+        const float d = in ? per_to_f32(qy.v[j]) : 0.f;
+        aw[k][j] = fmaf(d, h[k][j], aw[k][j]);
+        ab[k][j] += d;
+        gv[k][j] = g.w && in ? d * per_to_f32(w[k].v[j]) : d;
+        s1 += gv[k][j];
+        s2 = fmaf(gv[k][j], h[k][j], s2);
+      }
+    }
+    fetch(stage, row + R::kStages * t.step);
+    fetch_stats(row + t.step);
+    stage = stage + 1 == R::kStages ? 0 : stage + 1;
+    if (!g.dx) continue;
+    const float2 sum = row_sum2<LANES>(s1, s2, ex, turn);
+    const float c1 = sum.x / n, c2 = sum.y / n;
+    if (row < g.rows) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int c = (t.lane + k * t.width) * VEC;
+        if (c >= g.dim) continue;
+        Pack<T, VEC> o;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          o.v[j] = per_from_f32<T>(r * (gv[k][j] - c1 - h[k][j] * c2));
+        store<T, VEC>(dx + row * g.dx_stride + c, o);
+      }
+    }
+  }
+  if (!g.part) return;
+  if constexpr (LANES <= 0) {
+    float* part = g.part + t.base * 2 * g.dim;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (t.lane + k * t.width) * VEC;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        if (c < g.dim) {
+          part[c + j] = aw[k][j];
+          part[g.dim + c + j] = ab[k][j];
+        }
+    }
+  } else {
+    // the row groups of a warp by shuffles, then the warps through shared memory, where the
+    // (empty) copy groups still in flight have ended
+    float* part = g.part + (int64_t)blockIdx.x * 2 * g.dim;
+    float* sums = reinterpret_cast<float*>(dyn);  // [warps][2][dim]
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+#pragma unroll
+        for (int o = LANES; o < 32; o <<= 1) {
+          aw[k][j] += __shfl_xor_sync(PER_FULL_MASK, aw[k][j], o);
+          ab[k][j] += __shfl_xor_sync(PER_FULL_MASK, ab[k][j], o);
+        }
+        const int c = (t.lane + k * t.width) * VEC + j;
+        if (t.mine == 0 && c < g.dim) {
+          float* s = sums + (threadIdx.x >> 5) * 2 * g.dim;
+          s[c] = aw[k][j];
+          s[g.dim + c] = ab[k][j];
+        }
+      }
+    __syncthreads();
+    for (int c = threadIdx.x; c < 2 * g.dim; c += blockDim.x) {
+      float v = 0.f;
+      for (int q = 0; q < (int)(blockDim.x >> 5); ++q) v += sums[q * 2 * g.dim + c];
+      part[c] = v;
+    }
+  }
+}
+
 // ---- rows of any length: one CTA per row, the row read three times (from
 // L2 after the first)
 template <typename T, typename P>
@@ -153,30 +615,54 @@ __global__ void __launch_bounds__(kThreads) per_layer_norm_dw_long_kernel(const 
   g.part[((int64_t)split * 2 + 1) * g.dim + c] = db;
 }
 
-// dw and db from the splits' sums, added in order.
+// dw and db from the partial rows: a CTA adds 32 columns, each of its 8 warps
+// every eighth partial row, then the warps' sums in order.
+constexpr int kJoinThreads = 256;
 template <typename P>
-__global__ void __launch_bounds__(kThreads) per_layer_norm_join_kernel(const Bwd g) {
+__global__ void __launch_bounds__(kJoinThreads) per_layer_norm_join_kernel(const Bwd g) {
+  __shared__ float s[kJoinThreads / 32][32];
   per_wait_previous_grid();
-  const int64_t c = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (c >= g.dim) return;
-  float dw = 0.f, db = 0.f;
-  for (int k = 0; k < g.splits; ++k) {
-    dw += g.part[(int64_t)k * 2 * g.dim + c];
-    db += g.part[((int64_t)k * 2 + 1) * g.dim + c];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane;  // column of [dw, db]
+  const int64_t cols = 2 * (int64_t)g.dim;
+  float v = 0.f;
+  if (c < cols) {
+#pragma unroll 8
+    for (int k = warp; k < g.splits; k += kJoinThreads / 32) v += g.part[k * cols + c];
   }
-  if (g.dw) static_cast<P*>(g.dw)[c] = per_from_f32<P>(dw);
-  if (g.db) static_cast<P*>(g.db)[c] = per_from_f32<P>(db);
+  s[warp][lane] = v;
+  __syncthreads();
+  if (warp || c >= cols) return;
+#pragma unroll
+  for (int q = 1; q < kJoinThreads / 32; ++q) v += s[q][lane];
+  void* out = c < g.dim ? g.dw : g.db;
+  if (out) static_cast<P*>(out)[c < g.dim ? c : c - g.dim] = per_from_f32<P>(v);
 }
 
-int launch(const void* fn, int64_t grid, const void* arg, cudaStream_t stream) {
+int launch(const void* fn, int64_t grid, int threads, size_t smem, const void* arg,
+           cudaStream_t stream, int cluster = 1) {
   void* args[] = {const_cast<void*>(arg)};
-  const cudaError_t e = per_launch(fn, (unsigned)grid, kThreads, 0, stream, args, false);
+  const cudaError_t e = cluster > 1
+                            ? per_launch_cluster(fn, (unsigned)grid, threads, smem, cluster, stream, args)
+                            : per_launch(fn, (unsigned)grid, threads, smem, stream, args, false);
   return e == cudaSuccess ? PER_OK : per_record_cuda(e);
 }
 
 int64_t row_grid(int64_t rows) { return rows < 65535 ? rows : 65535; }
 
-// Row splits of the column sums.
+int sm_count() {
+  static int sms[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if (!sms[dev]) {
+    int v = 0;
+    if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) v = 148;
+    sms[dev] = v;
+  }
+  return sms[dev];
+}
+
+// Row splits of the column sums of long rows.
 int splits_of(int64_t rows, int64_t dim) {
   const int64_t tiles = (dim - 1) / kThreads + 1;
   int64_t s = 1184 / tiles;
@@ -185,21 +671,148 @@ int splits_of(int64_t rows, int64_t dim) {
   return s < 1 ? 1 : (int)s;
 }
 
+// How a row is laid over threads: `lanes` of a warp with `nv` vectors each, or
+// `ctas` CTAs of `threads` (lanes 0). ctas 0: too long for registers.
+struct Shape {
+  int lanes, nv, threads, ctas;
+};
+
+// A thread holds up to 8 values of a row, so that statistics, sums and
+// weights fit its registers at full occupancy of a CTA of 1024. Rows of up to
+// 32 x 8 values stay in a warp, which needs no barrier; rows of up to 1024 x 8
+// take a CTA, longer ones a cluster of up to 8.
+Shape shape_of(int64_t dim, int vec, int warp_threads) {
+  const int64_t v = (dim + vec - 1) / vec;
+  const int full = 8 / vec, small = vec == 1 ? 4 : 1, most = row_threads(vec);
+  for (int lanes = 4; lanes <= 32; lanes *= 2)
+    if (v <= lanes * small) return {lanes, small, warp_threads, 1};
+  if (v <= 32 * full) return {32, full, warp_threads, 1};
+  for (int ctas = 1; ctas <= kMaxCluster; ctas *= 2)
+    if (v <= (int64_t)ctas * most * full) {
+      const int64_t threads = (v + ctas * full - 1) / (ctas * full);
+      return {0, full, (int)((threads + 31) / 32 * 32), ctas};
+    }
+  return {0, 0, 0, 0};
+}
+
+// fn<..., VEC, NV, LANES>(shape, args) for the shape; false where there is none
+#define PER_NORM_SHAPE(s, rc, go, T, P, VEC, ...)                                              \
+  [&]() -> bool {                                                                              \
+    constexpr int kSmall = VEC == 1 ? 4 : 1, kFull = 8 / VEC;                                  \
+    if (s.lanes == 4) return rc = go<T, P, VEC, kSmall, 4>(s, __VA_ARGS__), true;              \
+    if (s.lanes == 8) return rc = go<T, P, VEC, kSmall, 8>(s, __VA_ARGS__), true;              \
+    if (s.lanes == 16) return rc = go<T, P, VEC, kSmall, 16>(s, __VA_ARGS__), true;            \
+    if (s.lanes == 32 && s.nv == kSmall)                                                       \
+      return rc = go<T, P, VEC, kSmall, 32>(s, __VA_ARGS__), true;                             \
+    if (s.lanes == 32) return rc = go<T, P, VEC, kFull, 32>(s, __VA_ARGS__), true;             \
+    if (s.ctas == 1) return rc = go<T, P, VEC, kFull, 0>(s, __VA_ARGS__), true;                \
+    if (s.ctas > 1) return rc = go<T, P, VEC, kFull, -1>(s, __VA_ARGS__), true;                \
+    return false;                                                                              \
+  }()
+
+bool aligned(const void* p, int64_t stride, size_t elem) {
+  return (uintptr_t)p % 16 == 0 && (stride * (int64_t)elem) % 16 == 0;
+}
+
+// CTAs (or clusters) that share `rows`: what is co-resident, or fewer.
+int row_ctas(const void* fn, const Shape& s, size_t smem, int64_t rows, int64_t most, int64_t* out) {
+  int rc = per_set_smem(fn, smem);
+  if (rc) return rc;
+  int ctas = 0;
+  rc = per_coresident_ctas(fn, s.threads, smem, &ctas);
+  if (rc) return rc;
+  const int64_t per_cta = s.lanes ? s.threads / s.lanes : 1;
+  int64_t grid = (rows - 1) / per_cta + 1;
+  const int64_t room = ctas / s.ctas > 0 ? ctas / s.ctas : 1;
+  if (grid > room) grid = room;
+  if (most > 0 && grid > most) grid = most;
+  *out = grid;
+  return PER_OK;
+}
+
+template <typename T, typename P, int VEC, int NV, int LANES>
+int forward_go(const Shape& s, const Fwd& f, cudaStream_t stream) {
+  const void* fn = (const void*)per_layer_norm_kernel<T, P, VEC, NV, LANES>;
+  const size_t smem = Ring<T, VEC, NV, kFwdStages>::kBytes * s.threads;
+  int64_t grid = 0;
+  const int rc = row_ctas(fn, s, smem, f.rows, 0, &grid);
+  if (rc) return rc;
+  return launch(fn, grid * s.ctas, s.threads, smem, &f, stream, s.ctas);
+}
+
+template <typename T, typename P, int VEC>
+int forward_vec(const Fwd& f, cudaStream_t stream) {
+  const Shape s = shape_of(f.dim, VEC, 128);
+  int rc = PER_OK;
+  if (PER_NORM_SHAPE(s, rc, forward_go, T, P, VEC, f, stream)) return rc;
+  return launch((const void*)per_layer_norm_long_kernel<T, P>, row_grid(f.rows), kThreads, 0, &f,
+                stream);
+}
+
 template <typename T, typename P>
 int forward(const Fwd& f, cudaStream_t stream) {
-  return launch((const void*)per_layer_norm_long_kernel<T, P>, row_grid(f.rows), &f, stream);
+  constexpr int VEC = 16 / sizeof(T);
+  if (f.dim % VEC == 0 && aligned(f.x, f.x_stride, sizeof(T)) &&
+      aligned(f.y, f.y_stride, sizeof(T)) && aligned(f.w, 0, 1) && aligned(f.b, 0, 1))
+    return forward_vec<T, P, VEC>(f, stream);
+  return forward_vec<T, P, 1>(f, stream);
+}
+
+// Most partial rows of dw and db (the workspace is sized before the pointers'
+// alignment is known, so this holds for every kernel).
+int64_t most_partials(int64_t rows, int64_t dim) {
+  const int64_t most = (int64_t)sm_count() * (dim <= 2048 ? 8 : 2);
+  return rows < most ? rows : most;
+}
+
+template <typename T, typename P, int VEC, int NV, int LANES>
+int backward_go(const Shape& s, const Bwd& in, cudaStream_t stream) {
+  Bwd g = in;
+  const void* fn = (const void*)per_layer_norm_backward_kernel<T, P, VEC, NV, LANES>;
+  size_t smem = Ring<T, VEC, 2 * NV, kBwdStages>::kBytes * s.threads;
+  if constexpr (LANES > 0) {
+    const size_t sums = (size_t)(s.threads / 32) * 2 * g.dim * 4;
+    smem = smem > sums ? smem : sums;
+  }
+  int64_t grid = 0;
+  int rc = row_ctas(fn, s, smem, g.rows, most_partials(g.rows, g.dim), &grid);
+  if (rc) return rc;
+  const bool columns = g.dw || g.db;
+  if (!columns) g.part = nullptr;
+  rc = launch(fn, grid * s.ctas, s.threads, smem, &g, stream, s.ctas);
+  if (rc || !columns) return rc;
+  g.splits = (int32_t)grid;
+  return launch((const void*)per_layer_norm_join_kernel<P>, (2 * (int64_t)g.dim - 1) / 32 + 1,
+                kJoinThreads, 0, &g, stream);
+}
+
+template <typename T, typename P, int VEC>
+int backward_vec(const Bwd& in, cudaStream_t stream) {
+  const Shape s = shape_of(in.dim, VEC, 256);
+  int rc = PER_OK;
+  if (PER_NORM_SHAPE(s, rc, backward_go, T, P, VEC, in, stream)) return rc;
+  Bwd g = in;
+  g.splits = splits_of(g.rows, g.dim);
+  if (g.dx)
+    rc = launch((const void*)per_layer_norm_dx_long_kernel<T, P>, row_grid(g.rows), kThreads, 0,
+                &g, stream);
+  if (rc || (!g.dw && !g.db)) return rc;
+  const int64_t tiles = (g.dim - 1) / kThreads + 1;
+  rc = launch((const void*)per_layer_norm_dw_long_kernel<T>, tiles * g.splits, kThreads, 0, &g,
+              stream);
+  if (rc) return rc;
+  return launch((const void*)per_layer_norm_join_kernel<P>, (2 * (int64_t)g.dim - 1) / 32 + 1,
+                kJoinThreads, 0, &g, stream);
 }
 
 template <typename T, typename P>
 int backward(const Bwd& g, cudaStream_t stream) {
-  int rc = PER_OK;
-  if (g.dx)
-    rc = launch((const void*)per_layer_norm_dx_long_kernel<T, P>, row_grid(g.rows), &g, stream);
-  if (rc || (!g.dw && !g.db)) return rc;
-  const int64_t tiles = (g.dim - 1) / kThreads + 1;
-  rc = launch((const void*)per_layer_norm_dw_long_kernel<T>, tiles * g.splits, &g, stream);
-  if (rc) return rc;
-  return launch((const void*)per_layer_norm_join_kernel<P>, tiles, &g, stream);
+  constexpr int VEC = 16 / sizeof(T);
+  if (g.dim % VEC == 0 && aligned(g.x, g.x_stride, sizeof(T)) &&
+      aligned(g.dy, g.dy_stride, sizeof(T)) && aligned(g.dx, g.dx_stride, sizeof(T)) &&
+      aligned(g.w, 0, 1))
+    return backward_vec<T, P, VEC>(g, stream);
+  return backward_vec<T, P, 1>(g, stream);
 }
 
 }  // namespace
@@ -221,7 +834,10 @@ int per_launch_layer_norm(const per_norm_t& n, const void* x, int64_t x_stride, 
 }
 
 int64_t per_layer_norm_backward_bytes(const per_norm_t& n) {
-  return (int64_t)splits_of(n.rows, n.dim) * 2 * n.dim * 4;
+  int64_t most = most_partials(n.rows, n.dim);
+  const int64_t s = splits_of(n.rows, n.dim);
+  if (most < s) most = s;
+  return most * 2 * n.dim * 4;
 }
 
 int per_launch_layer_norm_backward(const per_norm_t& n, const void* dy, int64_t dy_stride,
@@ -230,7 +846,6 @@ int per_launch_layer_norm_backward(const per_norm_t& n, const void* dy, int64_t 
                                    int64_t dx_stride, void* dweight, void* dbias, void* workspace,
                                    cudaStream_t stream) {
   const Bwd g{dy, x, weight, mean, rstd, dx, dweight, dbias, static_cast<float*>(workspace),
-              n.rows, dy_stride, x_stride, dx_stride, (int32_t)n.dim,
-              splits_of(n.rows, n.dim)};
+              n.rows, dy_stride, x_stride, dx_stride, (int32_t)n.dim, 0};
   return PER_NORM_TYPES(n, backward, g, stream);
 }
