@@ -46,6 +46,7 @@ struct Bwd {
   float* part;  // [splits][2][dim]
   int64_t rows, dy_stride, x_stride, dx_stride;
   int32_t dim, splits;
+  int32_t group_threads;  // of a row that spans warps
 };
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -65,6 +66,38 @@ __device__ __forceinline__ float2 block_sum2(float a, float b) {
   const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
   const float2 v = lane < warps ? s[lane] : make_float2(0.f, 0.f);
   return make_float2(warp_sum(v.x), warp_sum(v.y));
+}
+
+// Pairs of float32: one instruction for two additions, products or
+// multiply-adds, each rounded as the single operation is.
+__device__ __forceinline__ uint64_t bits(float2 a) {
+  return (uint64_t)__float_as_uint(a.x) | ((uint64_t)__float_as_uint(a.y) << 32);
+}
+__device__ __forceinline__ float2 pair(uint64_t u) {
+  return make_float2(__uint_as_float((uint32_t)u), __uint_as_float((uint32_t)(u >> 32)));
+}
+__device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)));
+  return pair(r);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)));
+  return pair(r);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
+  return pair(r);
+}
+
+// a / n for a count n, with inv = 1 / n: the first quotient corrected by its
+// exact remainder, so that an exact quotient comes out exact.
+__device__ __forceinline__ float over(float a, float n, float inv) {
+  const float q = a * inv;
+  return fmaf(fmaf(-q, n, a), inv, q);
 }
 
 // VEC values that are loaded and stored at once.
@@ -97,10 +130,22 @@ __device__ __forceinline__ void store(T* p, const Pack<T, VEC>& r) {
     *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(&r);
 }
 
+// The values of a thread, NV vectors of VEC, as pairs 0 .. NV VEC / 2.
+template <typename T, int VEC, int NV>
+__device__ __forceinline__ float2 get2(const Pack<T, VEC> (&p)[NV], int i) {
+  return make_float2(per_to_f32(p[2 * i / VEC].v[2 * i % VEC]),
+                     per_to_f32(p[(2 * i + 1) / VEC].v[(2 * i + 1) % VEC]));
+}
+template <typename T, int VEC, int NV>
+__device__ __forceinline__ void set2(Pack<T, VEC> (&p)[NV], int i, float2 f) {
+  p[2 * i / VEC].v[2 * i % VEC] = per_from_f32<T>(f.x);
+  p[(2 * i + 1) / VEC].v[(2 * i + 1) % VEC] = per_from_f32<T>(f.y);
+}
+
 // The threads of a row: LANES of them (a power of two, several rows per
-// warp), a whole CTA (LANES 0), or a cluster of CTAs (LANES -1, rows too long
-// for one). Thread `lane` of `width` holds the vectors lane, lane + width, ...
-// of VEC values, NV of them at most.
+// warp), a group of warps (LANES 0, one or several groups in a CTA), or a
+// cluster of CTAs (LANES -1, rows too long for one). Thread `lane` of `width`
+// holds the vectors lane, lane + width, ..., NV of them at most.
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -117,7 +162,11 @@ struct Row {
   int lane, width;     // of this thread in its row
   int64_t base, step;  // first row of this warp, rows between two of its turns
   int mine;            // this thread's row is base + mine
-  __device__ __forceinline__ Row() {
+  int group;           // of this CTA's groups
+  int warps;           // of a row that spans warps
+  __device__ __forceinline__ explicit Row(int group_threads) {
+    mine = group = 0;
+    warps = 1;
     if constexpr (LANES > 0) {
       const int per_cta = blockDim.x / LANES;
       lane = threadIdx.x % LANES;
@@ -125,13 +174,21 @@ struct Row {
       base = (int64_t)blockIdx.x * per_cta + (threadIdx.x & ~31) / LANES;
       step = (int64_t)gridDim.x * per_cta;
       mine = (threadIdx.x & 31) / LANES;
+    } else if constexpr (LANES == 0) {
+      const int groups = blockDim.x / group_threads;
+      group = threadIdx.x / group_threads;
+      lane = threadIdx.x - group * group_threads;
+      width = group_threads;
+      base = (int64_t)blockIdx.x * groups + group;
+      step = (int64_t)gridDim.x * groups;
+      warps = width >> 5;
     } else {
-      const int ctas = LANES == 0 ? 1 : (int)cluster_size();
-      lane = threadIdx.x + (LANES == 0 ? 0 : (int)(cluster_rank() * blockDim.x));
+      const int ctas = (int)cluster_size();
+      lane = threadIdx.x + (int)(cluster_rank() * blockDim.x);
       width = blockDim.x * ctas;
       base = blockIdx.x / ctas;
       step = gridDim.x / ctas;
-      mine = 0;
+      warps = width >> 5;
     }
   }
 };
@@ -148,27 +205,28 @@ __device__ __forceinline__ float lanes_sum(float v) {
 // per exchange is enough: a buffer is written again only after the barrier of
 // the next exchange, which follows every read of it.
 constexpr int kMaxCluster = 8;
+constexpr int kRowThreads = 512;  // of a CTA whose warps share rows
 template <int LANES>
 struct Exchange {
-  float3 slot[2][LANES == 0 ? 32 : 32 * kMaxCluster];
+  float4 slot[2][LANES == 0 ? kRowThreads / 32 : kRowThreads / 32 * kMaxCluster];
 };
 
 template <int LANES>
-__device__ __forceinline__ void put(Exchange<LANES>& e, int turn, float3 v) {
+__device__ __forceinline__ void put(Exchange<LANES>& e, int turn, const Row<LANES>& t, float4 v) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if constexpr (LANES == 0) {
     if (lane == 0) e.slot[turn][warp] = v;
-    __syncthreads();
+    __syncwarp();
+    asm volatile("bar.sync %0, %1;" ::"r"(t.group + 1), "r"(t.width) : "memory");
   } else {
-    const int ctas = (int)cluster_size();
-    if (lane < ctas) {  // lane = the CTA that the warp's words go to
-      const float3* at = &e.slot[turn][cluster_rank() * (blockDim.x >> 5) + warp];
+    if (lane < (int)cluster_size()) {  // lane = the CTA that the warp's words go to
+      const float4* at = &e.slot[turn][cluster_rank() * (blockDim.x >> 5) + warp];
       const uint32_t local = (uint32_t)__cvta_generic_to_shared(at);
       uint32_t remote;
       asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(lane));
-      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(v.x) : "memory");
-      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote + 4), "f"(v.y) : "memory");
-      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote + 8), "f"(v.z) : "memory");
+      asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(remote), "f"(v.x),
+                   "f"(v.y), "f"(v.z), "f"(v.w)
+                   : "memory");
     }
     __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -176,30 +234,28 @@ __device__ __forceinline__ void put(Exchange<LANES>& e, int turn, float3 v) {
   }
 }
 
-// Sums of a and b over the threads of a row.
+// The warps of a row as a lane sees them in an exchange: lane l reads warps
+// l mod span, + 32, ...; a butterfly over `span` lanes then joins them all.
 template <int LANES>
-__device__ __forceinline__ float2 row_sum2(float a, float b, Exchange<LANES>& e, int& turn) {
-  a = lanes_sum<LANES>(a);
-  b = lanes_sum<LANES>(b);
-  if constexpr (LANES > 0) {
-    return make_float2(a, b);
-  } else {
-    const int warps = (blockDim.x >> 5) * (LANES == 0 ? 1 : (int)cluster_size());
-    put<LANES>(e, turn, make_float3(a, b, 0.f));
-    a = b = 0.f;
-    for (int q = threadIdx.x & 31; q < warps; q += 32) {
-      a += e.slot[turn][q].x;
-      b += e.slot[turn][q].y;
-    }
-    turn ^= 1;
-    return make_float2(lanes_sum<0>(a), lanes_sum<0>(b));
+struct Warps {
+  static constexpr int kReads = LANES == 0 ? 1 : kRowThreads / 32 * kMaxCluster / 32;
+  int span, first, from;
+  __device__ __forceinline__ explicit Warps(const Row<LANES>& t) {
+    span = 1;
+    while (span < t.warps && span < 32) span *= 2;
+    first = threadIdx.x & (span - 1);
+    from = LANES == 0 ? t.group * t.warps : 0;
   }
-}
+  __device__ __forceinline__ float sum(float v) const {
+    for (int o = span >> 1; o; o >>= 1) v += __shfl_xor_sync(PER_FULL_MASK, v, o);
+    return v;
+  }
+};
 
 // A thread's own copies on their way into shared memory, STAGES rows ahead:
 // it waits for and reads only what it has copied itself, so no barrier is
 // needed. 16-byte vectors go by cp.async; single values are fetched into
-// registers one row ahead.
+// registers one row ahead. Where `in` is false the vector reads as zeros.
 template <typename T, int VEC, int NV, int STAGES>
 struct Ring {
   static constexpr bool kAsync = VEC * sizeof(T) == 16;
@@ -211,15 +267,18 @@ struct Ring {
   __device__ __forceinline__ explicit Ring(const void* smem) {
     at = (uint32_t)__cvta_generic_to_shared(smem) + threadIdx.x * 16;
   }
-  __device__ __forceinline__ void fetch(int stage, int k, const T* p, bool in) {
-    if (!in) return;
-    if constexpr (kAsync)
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+  // p is valid where `in` is true; base is always a valid address
+  __device__ __forceinline__ void fetch(int stage, int k, const T* base, int64_t offset, bool in) {
+    if constexpr (kAsync) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
                        at + (stage * NV + k) * blockDim.x * 16),
-                   "l"(p)
+                   "l"(in ? base + offset : base), "r"(in ? 16 : 0)
                    : "memory");
-    else
-      reg[k] = load<T, VEC>(p);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) reg[k].v[j] = per_from_f32<T>(0.f);
+      if (in) reg[k] = load<T, VEC>(base + offset);
+    }
   }
   static __device__ __forceinline__ void commit() {
     if constexpr (kAsync) asm volatile("cp.async.commit_group;" ::: "memory");
@@ -244,10 +303,6 @@ struct Ring {
   }
 };
 
-// Threads of a CTA that holds a row: 1024, or half of it for single values,
-// whose columns cost a thread more registers than 64.
-constexpr int row_threads(int vec) { return vec == 1 ? 512 : 1024; }
-
 // Before a CTA writes into another one's shared memory, that one has to run.
 template <int LANES>
 __device__ __forceinline__ void cluster_begins() {
@@ -257,138 +312,147 @@ __device__ __forceinline__ void cluster_begins() {
   }
 }
 
-constexpr int kFwdStages = 4;
+// weight (or its absence as 1, bias as 0) of this thread's columns
+template <typename P, int VEC, int NV>
+__device__ __forceinline__ void load_columns(Pack<P, VEC> (&w)[NV], const void* p, float absent,
+                                             int lane, int width, int dim) {
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = (lane + k * width) * VEC;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) w[k].v[j] = per_from_f32<P>(absent);
+    if (c < dim && p) w[k] = load<P, VEC>(static_cast<const P*>(p) + c);
+  }
+}
+
+constexpr int kFwdStages = 3;
 constexpr int kBwdStages = 3;
 
 // ---- forward, rows in registers
 template <typename T, typename P, int VEC, int NV, int LANES>
-__global__ void __launch_bounds__(LANES > 0 ? 128 : row_threads(VEC)) per_layer_norm_kernel(const Fwd f) {
+__global__ void __launch_bounds__(LANES > 0 ? 128 : kRowThreads) per_layer_norm_kernel(const Fwd f) {
   __shared__ Exchange<LANES> ex;
   extern __shared__ __align__(16) unsigned char dyn[];
-  const Row<LANES> t;
+  const Row<LANES> t(blockDim.x);
   using R = Ring<T, VEC, NV, kFwdStages>;
   R ring(dyn);
   int turn = 0, stage = 0;
-  const float n = (float)f.dim;
+  constexpr int E2 = NV * VEC / 2;
+  const float n = (float)f.dim, inv_n = 1.f / n;
   const T* x = static_cast<const T*>(f.x);
   T* y = static_cast<T*>(f.y);
-  int count = 0;  // values of this warp (of a row that spans warps)
+
+  // values of a warp (of a row that spans warps): this one's, and those of the
+  // warps that this lane reads in an exchange
+  const Warps<LANES> all(t);
+  auto values_of = [&](int warp) {
+    int v = 0;
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int c = (t.lane + k * t.width) * VEC;
-    count += c < f.dim ? VEC : 0;
+    for (int k = 0; k < NV; ++k) {
+      const int left = f.dim / VEC - warp * 32 - k * t.width;
+      v += left < 0 ? 0 : left > 32 ? 32 : left;
+    }
+    return (float)(v * VEC);
+  };
+  constexpr int Q = Warps<LANES>::kReads;
+  float own = n, mq[Q];
+  if constexpr (LANES <= 0) {
+    own = values_of(t.lane >> 5);
+#pragma unroll
+    for (int i = 0; i < Q; ++i)
+      mq[i] = all.first + 32 * i < t.warps ? values_of(all.first + 32 * i) : 0.f;
   }
-  if constexpr (LANES <= 0) count = __reduce_add_sync(PER_FULL_MASK, count);
+  const float inv_own = own > 0.f ? 1.f / own : 0.f;
+
   cluster_begins<LANES>();
   per_wait_previous_grid();
   auto fetch = [&](int st, int64_t row) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int c = (t.lane + k * t.width) * VEC;
-      ring.fetch(st, k, x + row * f.x_stride + c, row < f.rows && c < f.dim);
+      ring.fetch(st, k, x, row * f.x_stride + c, row < f.rows && c < f.dim);
     }
     R::commit();
   };
 #pragma unroll
   for (int k = 0; k < R::kStages; ++k) fetch(k, t.base + t.mine + k * t.step);
   Pack<P, VEC> w[NV], b[NV];
-#pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int c = (t.lane + k * t.width) * VEC;
-    if (c < f.dim && f.w) w[k] = load<P, VEC>(static_cast<const P*>(f.w) + c);
-    if (c < f.dim && f.b) b[k] = load<P, VEC>(static_cast<const P*>(f.b) + c);
-  }
+  load_columns(w, f.w, 1.f, t.lane, t.width, f.dim);
+  load_columns(b, f.b, 0.f, t.lane, t.width, f.dim);
   for (int64_t base = t.base; base < f.rows; base += t.step) {
     const int64_t row = base + t.mine;
-    float v[NV][VEC];
-    float a = 0.f;
+    float2 v[E2];
+    float2 a = both(0.f);
     R::wait();
+    {
+      Pack<T, VEC> q[NV];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const bool in = (t.lane + k * t.width) * VEC < f.dim;
-      const Pack<T, VEC> q = ring.get(stage, k);
+      for (int k = 0; k < NV; ++k) q[k] = ring.get(stage, k);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        v[k][j] = in ? per_to_f32(q.v[j]) : 0.f;
-        a += v[k][j];
+      for (int i = 0; i < E2; ++i) {
+        v[i] = get2(q, i);
+        a = add2(a, v[i]);
       }
     }
     fetch(stage, row + R::kStages * t.step);
     stage = stage + 1 == R::kStages ? 0 : stage + 1;
-    // distances from a first mean: the row's, or (rows that span warps) the warp's
-    const float own = LANES > 0 ? n : (float)count;
-    float s = lanes_sum<LANES>(a) / own;
-    if (LANES <= 0 && count == 0) s = 0.f;
-    float d1 = 0.f, d2 = 0.f;
+    // distances from a first mean: the row's, or (rows that span warps) the
+    // warp's; columns beyond the row, read as 0, stay at 0
+    const float s = over(lanes_sum<LANES>(a.x + a.y), own, inv_own);
+    float2 d1 = both(0.f), d2 = both(0.f);
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const bool in = (t.lane + k * t.width) * VEC < f.dim;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        v[k][j] = in ? v[k][j] - s : 0.f;
-        d1 += v[k][j];
-        d2 = fmaf(v[k][j], v[k][j], d2);
-      }
+    for (int i = 0; i < E2; ++i) {
+      const bool in0 = (t.lane + 2 * i / VEC * t.width) * VEC < f.dim;
+      const bool in1 = VEC > 1 ? in0 : (t.lane + (2 * i + 1) * t.width) < f.dim;
+      v[i] = add2(v[i], make_float2(in0 ? -s : 0.f, in1 ? -s : 0.f));
+      d1 = add2(d1, v[i]);
+      d2 = fma2(v[i], v[i], d2);
     }
-    d1 = lanes_sum<LANES>(d1);
-    d2 = lanes_sum<LANES>(d2);
-    float shift, var;      // h = (v - shift) r
+    const float e1 = lanes_sum<LANES>(d1.x + d1.y);
+    const float e2 = lanes_sum<LANES>(d2.x + d2.y);
+    float shift, var;  // h = (v - shift) r
     double mean;
     if constexpr (LANES > 0) {
-      shift = d1 / n;
-      var = d2 / n - shift * shift;
+      shift = over(e1, n, inv_n);
+      var = fmaf(-shift, shift, e2 * inv_n);
       mean = (double)s + (double)shift;
     } else {
-      // Warp q of m_q values: mean s_q + d1_q / m_q, squares around it d2_q - d1_q^2 / m_q. Seen
-      // from s_0 its mean lies at z_q; the row's at z = sum m_q z_q / n, and the row's squares are
-      // the warps' plus m_q (z_q - z)^2 each.
-      const int warps = (blockDim.x >> 5) * (LANES == 0 ? 1 : (int)cluster_size());
-      const float m1 = count ? d1 / own : 0.f;
-      put<LANES>(ex, turn, make_float3(s, m1, fmaxf(d2 - d1 * m1, 0.f)));
-      const float s0 = ex.slot[turn][0].x;
-      constexpr int Q = LANES == 0 ? 1 : kMaxCluster;
-      float z = 0.f, sq = 0.f, zq[Q], mq[Q];
+      // Warp q of m_q values: mean s_q + u_q with u_q = d1_q / m_q, squares around it
+      // d2_q - d1_q u_q. Seen from s_0 its mean lies at z_q; the row's at z = sum m_q z_q / n,
+      // and the row's squares are the warps' plus m_q (z_q - z)^2 each.
+      const float u = e1 * inv_own;
+      put<LANES>(ex, turn, t, make_float4(s, u, fmaxf(fmaf(-e1, u, e2), 0.f), 0.f));
+      const float s0 = ex.slot[turn][all.from].x;
+      float z = 0.f, sq = 0.f, zq[Q];
 #pragma unroll
       for (int i = 0; i < Q; ++i) {
-        const int q = (threadIdx.x & 31) + 32 * i;
-        zq[i] = mq[i] = 0.f;
-        if (q >= warps) continue;
-        const float3 o = ex.slot[turn][q];
-        // values of warp q: its vectors q * 32 + l + k width below dim / VEC
-        int vecs = 0;
-#pragma unroll
-        for (int k = 0; k < NV; ++k) {
-          const int left = f.dim / VEC - q * 32 - k * t.width;
-          vecs += left < 0 ? 0 : left > 32 ? 32 : left;
+        zq[i] = 0.f;
+        if (mq[i] > 0.f) {
+          const float4 o = ex.slot[turn][all.from + all.first + 32 * i];
+          zq[i] = (o.x - s0) + o.y;
+          sq += o.z;
         }
-        mq[i] = (float)(vecs * VEC);
-        zq[i] = vecs ? (o.x - s0) + o.y : 0.f;
         z = fmaf(mq[i], zq[i], z);
-        sq += o.z;
       }
       turn ^= 1;
-      z = lanes_sum<0>(z) / n;
+      z = over(all.sum(z), n, inv_n);
 #pragma unroll
       for (int i = 0; i < Q; ++i) sq = fmaf(mq[i] * (zq[i] - z), zq[i] - z, sq);
-      var = lanes_sum<0>(sq) / n;
+      var = all.sum(sq) * inv_n;
       shift = z - (s - s0);
       mean = (double)s0 + (double)z;
     }
     const float r = rsqrtf(fmaxf(var, 0.f) + f.eps);
+    const float2 r2 = both(r), c2 = both(-shift * r);
     if (row < f.rows) {
+      Pack<T, VEC> o[NV];
+#pragma unroll
+      for (int i = 0; i < E2; ++i)
+        set2(o, i, fma2(fma2(v[i], r2, c2), get2(w, i), get2(b, i)));
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         const int c = (t.lane + k * t.width) * VEC;
-        if (c >= f.dim) continue;
-        Pack<T, VEC> o;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          float h = (v[k][j] - shift) * r;
-          if (f.w) h *= per_to_f32(w[k].v[j]);
-          if (f.b) h += per_to_f32(b[k].v[j]);
-          o.v[j] = per_from_f32<T>(h);
-        }
-        store<T, VEC>(y + row * f.y_stride + c, o);
+        if (c < f.dim) store<T, VEC>(y + row * f.y_stride + c, o[k]);
       }
       if (f.mean && t.lane == 0) {
         f.mean[row] = mean;
@@ -399,18 +463,22 @@ __global__ void __launch_bounds__(LANES > 0 ? 128 : row_threads(VEC)) per_layer_
 }
 
 // ---- backward, rows in registers: dx, and the column sums of this CTA's
-// rows. Each thread keeps the sums of its columns while the CTA walks down
-// the rows; at the end the row groups of a CTA are joined in shared memory
-// and the CTA writes one partial row of dw and db.
+// rows. Each thread keeps the sums of its columns while its group walks down
+// the rows; at the end the groups of a CTA are joined in shared memory and
+// the CTA writes one partial row of dw and db. Columns beyond the row, and
+// rows beyond the last, read as dy = 0 and so add nothing to any sum.
 template <typename T, typename P, int VEC, int NV, int LANES>
-__global__ void __launch_bounds__(LANES > 0 ? 256 : row_threads(VEC)) per_layer_norm_backward_kernel(const Bwd g) {
+__global__ void __launch_bounds__(LANES > 0 ? 256 : kRowThreads)
+    per_layer_norm_backward_kernel(const Bwd g) {
   __shared__ Exchange<LANES> ex;
   extern __shared__ __align__(16) unsigned char dyn[];
-  const Row<LANES> t;
+  const Row<LANES> t(g.group_threads);
   using R = Ring<T, VEC, 2 * NV, kBwdStages>;
   R ring(dyn);
   int turn = 0, stage = 0;
-  const float n = (float)g.dim;
+  constexpr int E2 = NV * VEC / 2;
+  const float inv_n = 1.f / (float)g.dim;
+  const Warps<LANES> all(t);
   const T* x = static_cast<const T*>(g.x);
   const T* dy = static_cast<const T*>(g.dy);
   T* dx = static_cast<T*>(g.dx);
@@ -420,8 +488,9 @@ __global__ void __launch_bounds__(LANES > 0 ? 256 : row_threads(VEC)) per_layer_
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int c = (t.lane + k * t.width) * VEC;
-      ring.fetch(st, 2 * k, x + row * g.x_stride + c, row < g.rows && c < g.dim);
-      ring.fetch(st, 2 * k + 1, dy + row * g.dy_stride + c, row < g.rows && c < g.dim);
+      const bool in = row < g.rows && c < g.dim;
+      ring.fetch(st, k, x, row * g.x_stride + c, in);
+      ring.fetch(st, NV + k, dy, row * g.dy_stride + c, in);
     }
     R::commit();
   };
@@ -436,94 +505,107 @@ __global__ void __launch_bounds__(LANES > 0 ? 256 : row_threads(VEC)) per_layer_
   for (int k = 0; k < R::kStages; ++k) fetch(k, t.base + t.mine + k * t.step);
   fetch_stats(t.base + t.mine);
   Pack<P, VEC> w[NV];
-  float aw[NV][VEC], ab[NV][VEC];
+  load_columns(w, g.w, 1.f, t.lane, t.width, g.dim);
+  float2 aw[E2], ab[E2];
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int c = (t.lane + k * t.width) * VEC;
-    if (c < g.dim && g.w) w[k] = load<P, VEC>(static_cast<const P*>(g.w) + c);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) aw[k][j] = ab[k][j] = 0.f;
-  }
+  for (int i = 0; i < E2; ++i) aw[i] = ab[i] = both(0.f);
   for (int64_t base = t.base; base < g.rows; base += t.step) {
     const int64_t row = base + t.mine;
-    const float hi = (float)nm, lo = (float)(nm - (double)hi), r = nr;
-    float h[NV][VEC], gv[NV][VEC];
-    float s1 = 0.f, s2 = 0.f;
+    const float hi = (float)nm, r = nr;
+    const float lo = (float)(nm - (double)hi);
+    float2 h[E2], gv[E2];
+    float2 s1 = both(0.f), s2 = both(0.f);
     R::wait();
+    {
+      Pack<T, VEC> qx[NV], qy[NV];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const bool in = row < g.rows && (t.lane + k * t.width) * VEC < g.dim;
-      const Pack<T, VEC> qx = ring.get(stage, 2 * k), qy = ring.get(stage, 2 * k + 1);
+      for (int k = 0; k < NV; ++k) {
+        qx[k] = ring.get(stage, k);
+        qy[k] = ring.get(stage, NV + k);
+      }
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        h[k][j] = in ? (per_to_f32(qx.v[j]) - hi - lo) * r : 0.f;
-        const float d = in ? per_to_f32(qy.v[j]) : 0.f;
-        aw[k][j] = fmaf(d, h[k][j], aw[k][j]);
-        ab[k][j] += d;
-        gv[k][j] = g.w && in ? d * per_to_f32(w[k].v[j]) : d;
-        s1 += gv[k][j];
-        s2 = fmaf(gv[k][j], h[k][j], s2);
+      for (int i = 0; i < E2; ++i) {
+        const float2 d = get2(qy, i);
+        h[i] = fma2(add2(get2(qx, i), both(-hi)), both(r), both(-lo * r));
+        aw[i] = fma2(d, h[i], aw[i]);
+        ab[i] = add2(ab[i], d);
+        gv[i] = mul2(d, get2(w, i));
+        s1 = add2(s1, gv[i]);
+        s2 = fma2(gv[i], h[i], s2);
       }
     }
     fetch(stage, row + R::kStages * t.step);
     fetch_stats(row + t.step);
     stage = stage + 1 == R::kStages ? 0 : stage + 1;
     if (!g.dx) continue;
-    const float2 sum = row_sum2<LANES>(s1, s2, ex, turn);
-    const float c1 = sum.x / n, c2 = sum.y / n;
+    float a = lanes_sum<LANES>(s1.x + s1.y), q = lanes_sum<LANES>(s2.x + s2.y);
+    if constexpr (LANES <= 0) {
+      put<LANES>(ex, turn, t, make_float4(a, q, 0.f, 0.f));
+      a = q = 0.f;
+#pragma unroll
+      for (int i = 0; i < Warps<LANES>::kReads; ++i)
+        if (all.first + 32 * i < t.warps) {
+          const float4 o = ex.slot[turn][all.from + all.first + 32 * i];
+          a += o.x;
+          q += o.y;
+        }
+      turn ^= 1;
+      a = all.sum(a);
+      q = all.sum(q);
+    }
     if (row < g.rows) {
+      // r (g - a / n - h q / n)
+      const float2 r2 = both(r), k0 = both(-r * (a * inv_n)), k1 = both(-r * (q * inv_n));
+      Pack<T, VEC> o[NV];
+#pragma unroll
+      for (int i = 0; i < E2; ++i) set2(o, i, fma2(h[i], k1, fma2(gv[i], r2, k0)));
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         const int c = (t.lane + k * t.width) * VEC;
-        if (c >= g.dim) continue;
-        Pack<T, VEC> o;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j)
-          o.v[j] = per_from_f32<T>(r * (gv[k][j] - c1 - h[k][j] * c2));
-        store<T, VEC>(dx + row * g.dx_stride + c, o);
+        if (c < g.dim) store<T, VEC>(dx + row * g.dx_stride + c, o[k]);
       }
     }
   }
   if (!g.part) return;
-  if constexpr (LANES <= 0) {
+  if (LANES < 0 || (LANES == 0 && t.width == (int)blockDim.x)) {
     float* part = g.part + t.base * 2 * g.dim;
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int c = (t.lane + k * t.width) * VEC;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j)
-        if (c < g.dim) {
-          part[c + j] = aw[k][j];
-          part[g.dim + c + j] = ab[k][j];
-        }
+    for (int i = 0; i < E2; ++i) {
+      const int c0 = (t.lane + 2 * i / VEC * t.width) * VEC + 2 * i % VEC;
+      const int c1 = VEC > 1 ? c0 + 1 : t.lane + (2 * i + 1) * t.width;
+      if (c0 < g.dim) part[c0] = aw[i].x, part[g.dim + c0] = ab[i].x;
+      if (c1 < g.dim) part[c1] = aw[i].y, part[g.dim + c1] = ab[i].y;
     }
-  } else {
-    // the row groups of a warp by shuffles, then the warps through shared memory, where the
-    // (empty) copy groups still in flight have ended
+  } else if constexpr (LANES >= 0) {
+    // the row groups of a warp by shuffles, then the groups through shared
+    // memory, where the (empty) copies still in flight have ended
     float* part = g.part + (int64_t)blockIdx.x * 2 * g.dim;
-    float* sums = reinterpret_cast<float*>(dyn);  // [warps][2][dim]
+    float* sums = reinterpret_cast<float*>(dyn);  // [groups][2][dim]
+    const int group = LANES > 0 ? threadIdx.x >> 5 : t.group;
+    const int groups = LANES > 0 ? blockDim.x >> 5 : blockDim.x / t.width;
+    float* mine = sums + group * 2 * g.dim;
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
+    for (int i = 0; i < E2; ++i) {
+      if constexpr (LANES > 0) {
 #pragma unroll
         for (int o = LANES; o < 32; o <<= 1) {
-          aw[k][j] += __shfl_xor_sync(PER_FULL_MASK, aw[k][j], o);
-          ab[k][j] += __shfl_xor_sync(PER_FULL_MASK, ab[k][j], o);
-        }
-        const int c = (t.lane + k * t.width) * VEC + j;
-        if (t.mine == 0 && c < g.dim) {
-          float* s = sums + (threadIdx.x >> 5) * 2 * g.dim;
-          s[c] = aw[k][j];
-          s[g.dim + c] = ab[k][j];
+          aw[i].x += __shfl_xor_sync(PER_FULL_MASK, aw[i].x, o);
+          aw[i].y += __shfl_xor_sync(PER_FULL_MASK, aw[i].y, o);
+          ab[i].x += __shfl_xor_sync(PER_FULL_MASK, ab[i].x, o);
+          ab[i].y += __shfl_xor_sync(PER_FULL_MASK, ab[i].y, o);
         }
       }
+      const int c0 = (t.lane + 2 * i / VEC * t.width) * VEC + 2 * i % VEC;
+      const int c1 = VEC > 1 ? c0 + 1 : t.lane + (2 * i + 1) * t.width;
+      if (t.mine == 0 && c0 < g.dim) mine[c0] = aw[i].x, mine[g.dim + c0] = ab[i].x;
+      if (t.mine == 0 && c1 < g.dim) mine[c1] = aw[i].y, mine[g.dim + c1] = ab[i].y;
+    }
     __syncthreads();
     for (int c = threadIdx.x; c < 2 * g.dim; c += blockDim.x) {
       float v = 0.f;
-      for (int q = 0; q < (int)(blockDim.x >> 5); ++q) v += sums[q * 2 * g.dim + c];
+      for (int q = 0; q < groups; ++q) v += sums[q * 2 * g.dim + c];
       part[c] = v;
     }
   }
@@ -672,41 +754,56 @@ int splits_of(int64_t rows, int64_t dim) {
 }
 
 // How a row is laid over threads: `lanes` of a warp with `nv` vectors each, or
-// `ctas` CTAs of `threads` (lanes 0). ctas 0: too long for registers.
+// a group of `threads` of each of `ctas` CTAs (lanes 0). ctas 0: too long for
+// registers.
 struct Shape {
   int lanes, nv, threads, ctas;
 };
 
-// A thread holds up to 8 values of a row, so that statistics, sums and
-// weights fit its registers at full occupancy of a CTA of 1024. Rows of up to
-// 32 x 8 values stay in a warp, which needs no barrier; rows of up to 1024 x 8
-// take a CTA, longer ones a cluster of up to 8.
-Shape shape_of(int64_t dim, int vec, int warp_threads) {
+// Most vectors of a row that a thread holds. The sums over a row cost a thread
+// some 100 instructions whatever it holds, so it should hold much; statistics,
+// weights and (backward) two column sums per value have to fit its registers.
+template <typename T, int VEC>
+constexpr int fwd_vectors() {
+  return VEC == 1 ? 16 : 4;
+}
+template <typename T, int VEC>
+constexpr int bwd_vectors() {
+  return VEC == 1 ? 8 : sizeof(T) == 2 ? 2 : 4;
+}
+
+// Rows that a warp can hold stay in it, which needs no barrier; longer ones
+// take a group of warps, and beyond one CTA a cluster of up to 8.
+Shape shape_of(int64_t dim, int vec, int full, int warp_threads) {
   const int64_t v = (dim + vec - 1) / vec;
-  const int full = 8 / vec, small = vec == 1 ? 4 : 1, most = row_threads(vec);
+  const int small = vec == 1 ? 4 : 1;
   for (int lanes = 4; lanes <= 32; lanes *= 2)
     if (v <= lanes * small) return {lanes, small, warp_threads, 1};
-  if (v <= 32 * full) return {32, full, warp_threads, 1};
+  for (int nv = 2 * small; nv <= full; nv *= 2)
+    if (v <= 32 * nv) return {32, nv, warp_threads, 1};
   for (int ctas = 1; ctas <= kMaxCluster; ctas *= 2)
-    if (v <= (int64_t)ctas * most * full) {
+    if (v <= (int64_t)ctas * kRowThreads * full) {
       const int64_t threads = (v + ctas * full - 1) / (ctas * full);
       return {0, full, (int)((threads + 31) / 32 * 32), ctas};
     }
   return {0, 0, 0, 0};
 }
 
-// fn<..., VEC, NV, LANES>(shape, args) for the shape; false where there is none
-#define PER_NORM_SHAPE(s, rc, go, T, P, VEC, ...)                                              \
+// go<T, P, VEC, NV, LANES>(shape, ...) for the shape into rc; false where
+// there is none
+#define PER_NORM_SHAPE(s, rc, go, T, P, VEC, FULL, ...)                                        \
   [&]() -> bool {                                                                              \
-    constexpr int kSmall = VEC == 1 ? 4 : 1, kFull = 8 / VEC;                                  \
-    if (s.lanes == 4) return rc = go<T, P, VEC, kSmall, 4>(s, __VA_ARGS__), true;              \
-    if (s.lanes == 8) return rc = go<T, P, VEC, kSmall, 8>(s, __VA_ARGS__), true;              \
-    if (s.lanes == 16) return rc = go<T, P, VEC, kSmall, 16>(s, __VA_ARGS__), true;            \
-    if (s.lanes == 32 && s.nv == kSmall)                                                       \
-      return rc = go<T, P, VEC, kSmall, 32>(s, __VA_ARGS__), true;                             \
-    if (s.lanes == 32) return rc = go<T, P, VEC, kFull, 32>(s, __VA_ARGS__), true;             \
-    if (s.ctas == 1) return rc = go<T, P, VEC, kFull, 0>(s, __VA_ARGS__), true;                \
-    if (s.ctas > 1) return rc = go<T, P, VEC, kFull, -1>(s, __VA_ARGS__), true;                \
+    constexpr int S = VEC == 1 ? 4 : 1, F = FULL;                                              \
+    if (s.lanes == 4) return rc = go<T, P, VEC, S, 4>(s, __VA_ARGS__), true;                   \
+    if (s.lanes == 8) return rc = go<T, P, VEC, S, 8>(s, __VA_ARGS__), true;                   \
+    if (s.lanes == 16) return rc = go<T, P, VEC, S, 16>(s, __VA_ARGS__), true;                 \
+    if (s.lanes == 32 && s.nv == S) return rc = go<T, P, VEC, S, 32>(s, __VA_ARGS__), true;    \
+    if (s.lanes == 32 && s.nv == 2 * S)                                                        \
+      return rc = go<T, P, VEC, 2 * S, 32>(s, __VA_ARGS__), true;                              \
+    if constexpr (F >= 4 * S)                                                                  \
+      if (s.lanes == 32) return rc = go<T, P, VEC, 4 * S, 32>(s, __VA_ARGS__), true;           \
+    if (s.ctas == 1) return rc = go<T, P, VEC, F, 0>(s, __VA_ARGS__), true;                    \
+    if (s.ctas > 1) return rc = go<T, P, VEC, F, -1>(s, __VA_ARGS__), true;                    \
     return false;                                                                              \
   }()
 
@@ -715,13 +812,14 @@ bool aligned(const void* p, int64_t stride, size_t elem) {
 }
 
 // CTAs (or clusters) that share `rows`: what is co-resident, or fewer.
-int row_ctas(const void* fn, const Shape& s, size_t smem, int64_t rows, int64_t most, int64_t* out) {
+int row_ctas(const void* fn, const Shape& s, int threads, size_t smem, int64_t rows, int64_t most,
+             int64_t* out) {
   int rc = per_set_smem(fn, smem);
   if (rc) return rc;
   int ctas = 0;
-  rc = per_coresident_ctas(fn, s.threads, smem, &ctas);
+  rc = per_coresident_ctas(fn, threads, smem, &ctas);
   if (rc) return rc;
-  const int64_t per_cta = s.lanes ? s.threads / s.lanes : 1;
+  const int64_t per_cta = threads / (s.lanes ? s.lanes : s.threads);
   int64_t grid = (rows - 1) / per_cta + 1;
   const int64_t room = ctas / s.ctas > 0 ? ctas / s.ctas : 1;
   if (grid > room) grid = room;
@@ -735,16 +833,17 @@ int forward_go(const Shape& s, const Fwd& f, cudaStream_t stream) {
   const void* fn = (const void*)per_layer_norm_kernel<T, P, VEC, NV, LANES>;
   const size_t smem = Ring<T, VEC, NV, kFwdStages>::kBytes * s.threads;
   int64_t grid = 0;
-  const int rc = row_ctas(fn, s, smem, f.rows, 0, &grid);
+  const int rc = row_ctas(fn, s, s.threads, smem, f.rows, 0, &grid);
   if (rc) return rc;
   return launch(fn, grid * s.ctas, s.threads, smem, &f, stream, s.ctas);
 }
 
 template <typename T, typename P, int VEC>
 int forward_vec(const Fwd& f, cudaStream_t stream) {
-  const Shape s = shape_of(f.dim, VEC, 128);
+  constexpr int FULL = fwd_vectors<T, VEC>();
+  const Shape s = shape_of(f.dim, VEC, FULL, 128);
   int rc = PER_OK;
-  if (PER_NORM_SHAPE(s, rc, forward_go, T, P, VEC, f, stream)) return rc;
+  if (PER_NORM_SHAPE(s, rc, forward_go, T, P, VEC, FULL, f, stream)) return rc;
   return launch((const void*)per_layer_norm_long_kernel<T, P>, row_grid(f.rows), kThreads, 0, &f,
                 stream);
 }
@@ -761,7 +860,7 @@ int forward(const Fwd& f, cudaStream_t stream) {
 // Most partial rows of dw and db (the workspace is sized before the pointers'
 // alignment is known, so this holds for every kernel).
 int64_t most_partials(int64_t rows, int64_t dim) {
-  const int64_t most = (int64_t)sm_count() * (dim <= 2048 ? 8 : 2);
+  const int64_t most = (int64_t)sm_count() * (dim <= 512 ? 8 : dim <= 2048 ? 4 : 2);
   return rows < most ? rows : most;
 }
 
@@ -769,17 +868,21 @@ template <typename T, typename P, int VEC, int NV, int LANES>
 int backward_go(const Shape& s, const Bwd& in, cudaStream_t stream) {
   Bwd g = in;
   const void* fn = (const void*)per_layer_norm_backward_kernel<T, P, VEC, NV, LANES>;
-  size_t smem = Ring<T, VEC, 2 * NV, kBwdStages>::kBytes * s.threads;
-  if constexpr (LANES > 0) {
-    const size_t sums = (size_t)(s.threads / 32) * 2 * g.dim * 4;
+  // a CTA of about 256 threads: several groups share its partial row
+  const int groups = LANES == 0 && s.threads <= 128 ? 256 / s.threads : 1;
+  const int threads = s.threads * groups;
+  g.group_threads = s.threads;
+  size_t smem = Ring<T, VEC, 2 * NV, kBwdStages>::kBytes * threads;
+  if (LANES > 0 || groups > 1) {
+    const size_t sums = (size_t)(LANES > 0 ? threads / 32 : groups) * 2 * g.dim * 4;
     smem = smem > sums ? smem : sums;
   }
   int64_t grid = 0;
-  int rc = row_ctas(fn, s, smem, g.rows, most_partials(g.rows, g.dim), &grid);
+  int rc = row_ctas(fn, s, threads, smem, g.rows, most_partials(g.rows, g.dim), &grid);
   if (rc) return rc;
   const bool columns = g.dw || g.db;
   if (!columns) g.part = nullptr;
-  rc = launch(fn, grid * s.ctas, s.threads, smem, &g, stream, s.ctas);
+  rc = launch(fn, grid * s.ctas, threads, smem, &g, stream, s.ctas);
   if (rc || !columns) return rc;
   g.splits = (int32_t)grid;
   return launch((const void*)per_layer_norm_join_kernel<P>, (2 * (int64_t)g.dim - 1) / 32 + 1,
@@ -788,9 +891,10 @@ int backward_go(const Shape& s, const Bwd& in, cudaStream_t stream) {
 
 template <typename T, typename P, int VEC>
 int backward_vec(const Bwd& in, cudaStream_t stream) {
-  const Shape s = shape_of(in.dim, VEC, 256);
+  constexpr int FULL = bwd_vectors<T, VEC>();
+  const Shape s = shape_of(in.dim, VEC, FULL, 256);
   int rc = PER_OK;
-  if (PER_NORM_SHAPE(s, rc, backward_go, T, P, VEC, in, stream)) return rc;
+  if (PER_NORM_SHAPE(s, rc, backward_go, T, P, VEC, FULL, in, stream)) return rc;
   Bwd g = in;
   g.splits = splits_of(g.rows, g.dim);
   if (g.dx)
@@ -846,6 +950,6 @@ int per_launch_layer_norm_backward(const per_norm_t& n, const void* dy, int64_t 
                                    int64_t dx_stride, void* dweight, void* dbias, void* workspace,
                                    cudaStream_t stream) {
   const Bwd g{dy, x, weight, mean, rstd, dx, dweight, dbias, static_cast<float*>(workspace),
-              n.rows, dy_stride, x_stride, dx_stride, (int32_t)n.dim, 0};
+              n.rows, dy_stride, x_stride, dx_stride, (int32_t)n.dim, 0, 0};
   return PER_NORM_TYPES(n, backward, g, stream);
 }
