@@ -68,31 +68,6 @@ __device__ __forceinline__ float2 block_sum2(float a, float b) {
   return make_float2(warp_sum(v.x), warp_sum(v.y));
 }
 
-// Pairs of float32: one instruction for two additions, products or
-// multiply-adds, each rounded as the single operation is.
-__device__ __forceinline__ uint64_t bits(float2 a) {
-  return (uint64_t)__float_as_uint(a.x) | ((uint64_t)__float_as_uint(a.y) << 32);
-}
-__device__ __forceinline__ float2 pair(uint64_t u) {
-  return make_float2(__uint_as_float((uint32_t)u), __uint_as_float((uint32_t)(u >> 32)));
-}
-__device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)));
-  return pair(r);
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)));
-  return pair(r);
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
-  return pair(r);
-}
-
 // a / n for a count n, with inv = 1 / n: the first quotient corrected by its
 // exact remainder, so that an exact quotient comes out exact.
 __device__ __forceinline__ float over(float a, float n, float inv) {
@@ -130,16 +105,27 @@ __device__ __forceinline__ void store(T* p, const Pack<T, VEC>& r) {
     *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(&r);
 }
 
-// The values of a thread, NV vectors of VEC, as pairs 0 .. NV VEC / 2.
-template <typename T, int VEC, int NV>
+// The values of a thread, NV vectors of VEC, as pairs 0 .. NV VEC / 2. WORDS:
+// taken from and put into whole 32-bit words, which costs fewer instructions;
+// the forward kernel goes by single values, because from words the compiler
+// keeps weight and bias unpacked across rows and spills (65536x4096 bfloat16:
+// 178 us by values, 203 by words; backward 304 us by values, 290 by words).
+template <bool WORDS, typename T, int VEC, int NV>
 __device__ __forceinline__ float2 get2(const Pack<T, VEC> (&p)[NV], int i) {
-  return make_float2(per_to_f32(p[2 * i / VEC].v[2 * i % VEC]),
-                     per_to_f32(p[(2 * i + 1) / VEC].v[(2 * i + 1) % VEC]));
+  if constexpr (WORDS && sizeof(T) == 2 && VEC > 1)
+    return per_unpack<T>(reinterpret_cast<const uint32_t*>(&p[2 * i / VEC])[i % (VEC / 2)]);
+  else
+    return make_float2(per_to_f32(p[2 * i / VEC].v[2 * i % VEC]),
+                       per_to_f32(p[(2 * i + 1) / VEC].v[(2 * i + 1) % VEC]));
 }
-template <typename T, int VEC, int NV>
+template <bool WORDS, typename T, int VEC, int NV>
 __device__ __forceinline__ void set2(Pack<T, VEC> (&p)[NV], int i, float2 f) {
-  p[2 * i / VEC].v[2 * i % VEC] = per_from_f32<T>(f.x);
-  p[(2 * i + 1) / VEC].v[(2 * i + 1) % VEC] = per_from_f32<T>(f.y);
+  if constexpr (WORDS && sizeof(T) == 2 && VEC > 1) {
+    reinterpret_cast<uint32_t*>(&p[2 * i / VEC])[i % (VEC / 2)] = per_pack<T>(f);
+  } else {
+    p[2 * i / VEC].v[2 * i % VEC] = per_from_f32<T>(f.x);
+    p[(2 * i + 1) / VEC].v[(2 * i + 1) % VEC] = per_from_f32<T>(f.y);
+  }
 }
 
 // The threads of a row: LANES of them (a power of two, several rows per
@@ -382,7 +368,7 @@ __global__ void __launch_bounds__(LANES > 0 ? 128 : kRowThreads) per_layer_norm_
   for (int64_t base = t.base; base < f.rows; base += t.step) {
     const int64_t row = base + t.mine;
     float2 v[E2];
-    float2 a = both(0.f);
+    float2 a = per_both(0.f);
     R::wait();
     {
       Pack<T, VEC> q[NV];
@@ -390,8 +376,8 @@ __global__ void __launch_bounds__(LANES > 0 ? 128 : kRowThreads) per_layer_norm_
       for (int k = 0; k < NV; ++k) q[k] = ring.get(stage, k);
 #pragma unroll
       for (int i = 0; i < E2; ++i) {
-        v[i] = get2(q, i);
-        a = add2(a, v[i]);
+        v[i] = get2<false>(q, i);
+        a = per_add2(a, v[i]);
       }
     }
     fetch(stage, row + R::kStages * t.step);
@@ -399,14 +385,14 @@ __global__ void __launch_bounds__(LANES > 0 ? 128 : kRowThreads) per_layer_norm_
     // distances from a first mean: the row's, or (rows that span warps) the
     // warp's; columns beyond the row, read as 0, stay at 0
     const float s = over(lanes_sum<LANES>(a.x + a.y), own, inv_own);
-    float2 d1 = both(0.f), d2 = both(0.f);
+    float2 d1 = per_both(0.f), d2 = per_both(0.f);
 #pragma unroll
     for (int i = 0; i < E2; ++i) {
       const bool in0 = (t.lane + 2 * i / VEC * t.width) * VEC < f.dim;
       const bool in1 = VEC > 1 ? in0 : (t.lane + (2 * i + 1) * t.width) < f.dim;
-      v[i] = add2(v[i], make_float2(in0 ? -s : 0.f, in1 ? -s : 0.f));
-      d1 = add2(d1, v[i]);
-      d2 = fma2(v[i], v[i], d2);
+      v[i] = per_add2(v[i], make_float2(in0 ? -s : 0.f, in1 ? -s : 0.f));
+      d1 = per_add2(d1, v[i]);
+      d2 = per_fma2(v[i], v[i], d2);
     }
     const float e1 = lanes_sum<LANES>(d1.x + d1.y);
     const float e2 = lanes_sum<LANES>(d2.x + d2.y);
@@ -443,12 +429,12 @@ __global__ void __launch_bounds__(LANES > 0 ? 128 : kRowThreads) per_layer_norm_
       mean = (double)s0 + (double)z;
     }
     const float r = rsqrtf(fmaxf(var, 0.f) + f.eps);
-    const float2 r2 = both(r), c2 = both(-shift * r);
+    const float2 r2 = per_both(r), c2 = per_both(-shift * r);
     if (row < f.rows) {
       Pack<T, VEC> o[NV];
 #pragma unroll
       for (int i = 0; i < E2; ++i)
-        set2(o, i, fma2(fma2(v[i], r2, c2), get2(w, i), get2(b, i)));
+        set2<false>(o, i, per_fma2(per_fma2(v[i], r2, c2), get2<false>(w, i), get2<false>(b, i)));
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         const int c = (t.lane + k * t.width) * VEC;
@@ -508,13 +494,13 @@ __global__ void __launch_bounds__(LANES > 0 ? 256 : kRowThreads)
   load_columns(w, g.w, 1.f, t.lane, t.width, g.dim);
   float2 aw[E2], ab[E2];
 #pragma unroll
-  for (int i = 0; i < E2; ++i) aw[i] = ab[i] = both(0.f);
+  for (int i = 0; i < E2; ++i) aw[i] = ab[i] = per_both(0.f);
   for (int64_t base = t.base; base < g.rows; base += t.step) {
     const int64_t row = base + t.mine;
     const float hi = (float)nm, r = nr;
     const float lo = (float)(nm - (double)hi);
     float2 h[E2], gv[E2];
-    float2 s1 = both(0.f), s2 = both(0.f);
+    float2 s1 = per_both(0.f), s2 = per_both(0.f);
     R::wait();
     {
       Pack<T, VEC> qx[NV], qy[NV];
@@ -525,13 +511,13 @@ __global__ void __launch_bounds__(LANES > 0 ? 256 : kRowThreads)
       }
 #pragma unroll
       for (int i = 0; i < E2; ++i) {
-        const float2 d = get2(qy, i);
-        h[i] = fma2(add2(get2(qx, i), both(-hi)), both(r), both(-lo * r));
-        aw[i] = fma2(d, h[i], aw[i]);
-        ab[i] = add2(ab[i], d);
-        gv[i] = mul2(d, get2(w, i));
-        s1 = add2(s1, gv[i]);
-        s2 = fma2(gv[i], h[i], s2);
+        const float2 d = get2<true>(qy, i);
+        h[i] = per_fma2(per_add2(get2<true>(qx, i), per_both(-hi)), per_both(r), per_both(-lo * r));
+        aw[i] = per_fma2(d, h[i], aw[i]);
+        ab[i] = per_add2(ab[i], d);
+        gv[i] = per_mul2(d, get2<true>(w, i));
+        s1 = per_add2(s1, gv[i]);
+        s2 = per_fma2(gv[i], h[i], s2);
       }
     }
     fetch(stage, row + R::kStages * t.step);
@@ -555,10 +541,10 @@ __global__ void __launch_bounds__(LANES > 0 ? 256 : kRowThreads)
     }
     if (row < g.rows) {
       // r (g - a / n - h q / n)
-      const float2 r2 = both(r), k0 = both(-r * (a * inv_n)), k1 = both(-r * (q * inv_n));
+      const float2 r2 = per_both(r), k0 = per_both(-r * (a * inv_n)), k1 = per_both(-r * (q * inv_n));
       Pack<T, VEC> o[NV];
 #pragma unroll
-      for (int i = 0; i < E2; ++i) set2(o, i, fma2(h[i], k1, fma2(gv[i], r2, k0)));
+      for (int i = 0; i < E2; ++i) set2<true>(o, i, per_fma2(h[i], k1, per_fma2(gv[i], r2, k0)));
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         const int c = (t.lane + k * t.width) * VEC;

@@ -256,8 +256,11 @@ Tensor layer_norm(const Tensor& x, const std::vector<int64_t>& normalized_shape,
 // The list as the C ABI takes it; checks type, device and memory layout.
 // `writes`: also that no two tensors share memory.
 struct List {
-  std::vector<Tensor> keep;
+  // borrowed: the caller's list holds them (or the parameters whose gradients
+  // they are), and the GIL is held until the call's work is enqueued
+  std::vector<at::TensorImpl*> impl;
   std::vector<per_tensor_t> t;
+  c10::Device device{c10::kCPU};
 
   void add(const Tensor& g, const char* what) {
     if (!g.is_cuda())
@@ -268,13 +271,16 @@ struct List {
     const int32_t code = code_of(g.scalar_type());
     if (code < 0)
       throw py::type_error(std::string(what) + ": gradients must be float32, bfloat16 or float16");
-    if (!keep.empty() && g.device() != keep[0].device())
+    if (t.empty())
+      device = g.device();
+    else if (g.device() != device)
       throw py::value_error(std::string(what) + ": gradients must be on one device");
     if (!g.is_non_overlapping_and_dense())
       throw py::value_error(std::string(what) +
                             ": gradients must fill their memory without gaps or overlaps");
-    keep.push_back(g);
-    t.push_back(per_tensor_t{g.numel() ? g.data_ptr() : nullptr, g.numel(), code, 0});
+    impl.push_back(g.unsafeGetTensorImpl());
+    const int64_t n = g.numel();
+    t.push_back(per_tensor_t{n ? g.data_ptr() : nullptr, n, code, 0});
   }
 
   void check_disjoint(const char* what) const {
@@ -294,21 +300,22 @@ struct List {
                                                   "listed twice?)");
   }
 
-  void* stream() const { return stream_of(keep[0]); }
-  at::TensorOptions options() const { return keep[0].options(); }
+  void* stream() const { return c10::cuda::getCurrentCUDAStream(device.index()).stream(); }
+  at::TensorOptions options() const { return at::TensorOptions().device(device); }
   // the tensors have been written to
   void written() const {
-    for (const auto& g : keep)
-      if (!g.is_inference()) g.unsafeGetTensorImpl()->bump_version();
+    for (at::TensorImpl* g : impl)
+      if (!g->is_inference()) g->bump_version();
   }
 };
 
 List list_of(const py::list& tensors, bool take_grads, const char* what) {
   List l;
-  l.keep.reserve(tensors.size());
+  l.impl.reserve(tensors.size());
   l.t.reserve(tensors.size());
   for (const py::handle& h : tensors) {
-    const Tensor v = py::cast<Tensor>(h);
+    if (!THPVariable_Check(h.ptr())) throw py::type_error(std::string(what) + ": expected tensors");
+    const Tensor& v = THPVariable_Unpack(h.ptr());
     if (!take_grads) {
       l.add(v, what);
     } else if (v.grad().defined()) {
@@ -328,7 +335,7 @@ std::pair<Tensor, Tensor> norm_and_workspace(const List& l, int64_t* bytes) {
 py::object grad_norm(const py::list& tensors, bool take_grads, int kind) {
   const List l = list_of(tensors, take_grads, "grad_norm");
   if (l.t.empty()) return py::none();
-  c10::cuda::CUDAGuard guard(l.keep[0].device());
+  c10::cuda::CUDAGuard guard(l.device);
   int64_t bytes = 0;
   auto [norm, ws] = norm_and_workspace(l, &bytes);
   check("per_grad_norm", per_grad_norm(l.t.data(), (int64_t)l.t.size(), kind,
@@ -340,7 +347,7 @@ py::object clip_grad_norm(const py::list& params, int kind, double max_norm) {
   const List l = list_of(params, true, "clip_grad_norm_");
   if (l.t.empty()) return py::none();
   l.check_disjoint("clip_grad_norm_");
-  c10::cuda::CUDAGuard guard(l.keep[0].device());
+  c10::cuda::CUDAGuard guard(l.device);
   int64_t bytes = 0;
   auto [norm, ws] = norm_and_workspace(l, &bytes);
   check("per_clip_grad_norm",
@@ -354,14 +361,14 @@ void clip_grads_with_norm(const py::list& params, double max_norm, const Tensor&
   const List l = list_of(params, true, "clip_grads_with_norm_");
   if (l.t.empty()) return;
   l.check_disjoint("clip_grads_with_norm_");
-  if (norm.device() != l.keep[0].device() || norm.scalar_type() != at::kFloat || norm.numel() != 1)
+  if (norm.device() != l.device || norm.scalar_type() != at::kFloat || norm.numel() != 1)
     throw py::value_error("clip_grads_with_norm_: total_norm must be one float32 value on the "
                           "gradients' device");
   for (const auto& e : l.t)
     if (e.count && (uintptr_t)norm.data_ptr() >= (uintptr_t)e.data &&
         (uintptr_t)norm.data_ptr() < (uintptr_t)e.data + (uintptr_t)e.count * (e.dtype == PER_F32 ? 4 : 2))
       throw py::value_error("clip_grads_with_norm_: total_norm must not be part of a gradient");
-  c10::cuda::CUDAGuard guard(l.keep[0].device());
+  c10::cuda::CUDAGuard guard(l.device);
   check("per_scale_grads", per_scale_grads(l.t.data(), (int64_t)l.t.size(), (float)max_norm,
                                            norm.data_ptr<float>(), l.stream()));
   l.written();
