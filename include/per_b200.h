@@ -339,12 +339,13 @@ typedef struct per_norm {
  * of row r and rstd_r = 1 / sqrt(var_r + eps), var_r the mean squared
  * distance from m_r. Strides are in elements between the starts of rows
  * (>= dim), any alignment of the element size. weight and / or bias may be
- * NULL (1 and 0). mean (float64[rows]) and rstd (float32[rows]) receive the
- * rows' statistics for per_layer_norm_backward(); pass NULL for both when no
- * backward pass follows. y must not overlap x. */
+ * NULL (1 and 0). stats (float32[rows][4], 16-byte aligned) receives the rows'
+ * statistics for per_layer_norm_backward(): the mean as the sum of two floats
+ * (a mean rounded to one float would cost (x - mean) * rstd as many units of
+ * rounding as the mean is standard deviations), rstd, 0. NULL when no backward
+ * pass follows. y must not overlap x. */
 int per_layer_norm(const per_norm_t* norm, const void* x, int64_t x_stride, const void* weight,
-                   const void* bias, void* y, int64_t y_stride, double* mean, float* rstd,
-                   void* stream);
+                   const void* bias, void* y, int64_t y_stride, float* stats, void* stream);
 
 /* Bytes of `workspace` (16-byte aligned) that per_layer_norm_backward() needs
  * on the current device for this norm; -1 for a bad descriptor. */
@@ -361,9 +362,8 @@ int64_t per_layer_norm_backward_workspace(const per_norm_t* norm);
  * GPU need one each. Outputs must not overlap inputs. */
 int per_layer_norm_backward(const per_norm_t* norm, const void* dy, int64_t dy_stride,
                             const void* x, int64_t x_stride, const void* weight,
-                            const double* mean, const float* rstd, void* dx, int64_t dx_stride,
-                            void* dweight, void* dbias, void* workspace, int64_t workspace_bytes,
-                            void* stream);
+                            const float* stats, void* dx, int64_t dx_stride, void* dweight,
+                            void* dbias, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* One tensor of a list: `count` values of one type, dense in memory, in any
  * order (a norm does not depend on it). */

@@ -60,27 +60,26 @@ def test_structs_match_the_header():
 ])
 def test_layer_norm_refuses_bad_descriptors(kw, code):
     d = norm(**kw)
-    assert L.per_layer_norm(ctypes.byref(d), P, 8, None, None, 2 * P, 8, None, None, None) == code
+    assert L.per_layer_norm(ctypes.byref(d), P, 8, None, None, 2 * P, 8, None, None) == code
 
 
 def test_layer_norm_refuses_bad_pointers_and_strides():
     d = norm()
     f = lambda *a: L.per_layer_norm(ctypes.byref(d), *a, None)  # noqa: E731
-    assert L.per_layer_norm(None, P, 8, None, None, 2 * P, 8, None, None, None) == NULL
-    assert f(None, 8, None, None, 2 * P, 8, None, None) == NULL
-    assert f(P, 8, None, None, None, 8, None, None) == NULL
-    assert f(P, 8, None, None, 2 * P, 8, 3 * P, None) == NULL      # mean without rstd
-    assert f(P, 7, None, None, 2 * P, 8, None, None) == INVALID    # rows would overlap
-    assert f(P, 8, None, None, 2 * P, 7, None, None) == INVALID
-    assert f(P + 2, 8, None, None, 2 * P, 8, None, None) == MISALIGNED
-    assert f(P, 8, None, 3 * P + 1, 2 * P, 8, None, None) == MISALIGNED
-    assert f(P, 8, None, None, 2 * P, 8, 3 * P + 4, 4 * P) == MISALIGNED
-    assert f(P, 8, None, None, P, 8, None, None) == INVALID        # in place
-    assert f(P, 8, None, None, P + 3 * 32, 8, None, None) == INVALID
-    assert f(P, 16, None, None, P + 28, 16, None, None) == INVALID  # columns 7..15 over 0..8
-    assert f(P, 16, None, None, P - 28, 16, None, None) == INVALID
+    assert L.per_layer_norm(None, P, 8, None, None, 2 * P, 8, None, None) == NULL
+    assert f(None, 8, None, None, 2 * P, 8, None) == NULL
+    assert f(P, 8, None, None, None, 8, None) == NULL
+    assert f(P, 7, None, None, 2 * P, 8, None) == INVALID    # rows would overlap
+    assert f(P, 8, None, None, 2 * P, 7, None) == INVALID
+    assert f(P + 2, 8, None, None, 2 * P, 8, None) == MISALIGNED
+    assert f(P, 8, None, 3 * P + 1, 2 * P, 8, None) == MISALIGNED
+    assert f(P, 8, None, None, 2 * P, 8, 3 * P + 8) == MISALIGNED
+    assert f(P, 8, None, None, P, 8, None) == INVALID        # in place
+    assert f(P, 8, None, None, P + 3 * 32, 8, None) == INVALID
+    assert f(P, 16, None, None, P + 28, 16, None) == INVALID  # columns 7..15 over 0..8
+    assert f(P, 16, None, None, P - 28, 16, None) == INVALID
     empty = norm(rows=0)
-    assert L.per_layer_norm(ctypes.byref(empty), None, 8, None, None, None, 8, None, None, None) == OK
+    assert L.per_layer_norm(ctypes.byref(empty), None, 8, None, None, None, 8, None, None) == OK
 
 
 def test_layer_norm_backward_refuses_bad_calls():
@@ -89,13 +88,13 @@ def test_layer_norm_backward_refuses_bad_calls():
     assert need >= 0
     big = max(need, 1 << 20)
 
-    def f(dy=P, ds=8, x=2 * P, xs=8, w=None, mean=3 * P, rstd=4 * P, dx=5 * P, dxs=8, dw=6 * P,
+    def f(dy=P, ds=8, x=2 * P, xs=8, w=None, stats=3 * P, dx=5 * P, dxs=8, dw=6 * P,
           db=7 * P, ws=8 * P, nbytes=big, desc=d):
-        return L.per_layer_norm_backward(ctypes.byref(desc), dy, ds, x, xs, w, mean, rstd, dx, dxs,
+        return L.per_layer_norm_backward(ctypes.byref(desc), dy, ds, x, xs, w, stats, dx, dxs,
                                          dw, db, ws, nbytes, None)
 
     assert f(dx=None, dw=None, db=None) == OK  # nothing wanted
-    for name in ("dy", "x", "mean", "rstd"):
+    for name in ("dy", "x", "stats"):
         assert f(**{name: None}) == NULL, name
     if need:
         assert f(ws=None) == NULL
@@ -109,7 +108,7 @@ def test_layer_norm_backward_refuses_bad_calls():
     assert f(dx=2 * P) == INVALID  # over x
     assert f(ws=8 * P + 4) == MISALIGNED
     assert f(dw=6 * P + 2) == MISALIGNED
-    assert f(mean=3 * P + 4) == MISALIGNED
+    assert f(stats=3 * P + 8) == MISALIGNED
     assert f(desc=norm(dtype=5)) == INVALID
     assert L.per_layer_norm_backward_workspace(ctypes.byref(norm(dim=0))) == -1
     assert L.per_layer_norm_backward_workspace(None) == -1

@@ -18,6 +18,7 @@ struct OccEntry {
   const void* fn;
   int threads;
   size_t smem;
+  int cluster;
   int ctas;
 };
 constexpr int kOccSlots = 1024;
@@ -126,6 +127,10 @@ int per_record_cuda(cudaError_t e) {
 }
 
 int per_coresident_ctas(const void* fn, int threads, size_t smem, int* out) {
+  return per_coresident_clusters(fn, threads, smem, 1, out);
+}
+
+int per_coresident_clusters(const void* fn, int threads, size_t smem, int cluster, int* out) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return per_record_cuda(e);
@@ -133,22 +138,39 @@ int per_coresident_ctas(const void* fn, int threads, size_t smem, int* out) {
     std::lock_guard<std::mutex> lk(g_occ_mu);
     for (int i = 0; i < g_occ_n; ++i) {
       const OccEntry& o = g_occ[i];
-      if (o.device == dev && o.fn == fn && o.threads == threads && o.smem == smem) {
+      if (o.device == dev && o.fn == fn && o.threads == threads && o.smem == smem &&
+          o.cluster == cluster) {
         *out = o.ctas;
         return PER_OK;
       }
     }
   }
-  int sms = 0, per_sm = 0;
-  e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  if (e != cudaSuccess) return per_record_cuda(e);
-  e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, fn, threads, smem);
-  if (e != cudaSuccess) return per_record_cuda(e);
-  if (per_sm < 1) return PER_ERR_TOO_LARGE;
-  const int ctas = sms * per_sm;
+  int ctas = 0;
+  if (cluster > 1) {
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = cluster;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(cluster);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    e = cudaOccupancyMaxActiveClusters(&ctas, fn, &cfg);
+    if (e != cudaSuccess) return per_record_cuda(e);
+  } else {
+    int sms = 0, per_sm = 0;
+    e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return per_record_cuda(e);
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, fn, threads, smem);
+    if (e != cudaSuccess) return per_record_cuda(e);
+    ctas = sms * per_sm;
+  }
+  if (ctas < 1) return PER_ERR_TOO_LARGE;
   {
     std::lock_guard<std::mutex> lk(g_occ_mu);
-    if (g_occ_n < kOccSlots) g_occ[g_occ_n++] = OccEntry{dev, fn, threads, smem, ctas};
+    if (g_occ_n < kOccSlots) g_occ[g_occ_n++] = OccEntry{dev, fn, threads, smem, cluster, ctas};
   }
   *out = ctas;
   return PER_OK;

@@ -29,6 +29,11 @@ int per_check_store(const per_store_t* s, bool with_scratch);
 // all co-resident on the current device; cached per (device, fn, smem).
 int per_coresident_ctas(const void* fn, int threads, size_t smem, int* out);
 
+// The same in clusters of `cluster` CTAs: how many clusters are co-resident.
+// Fewer than the CTAs would allow, because a cluster stays within one of the
+// GPU's processing clusters.
+int per_coresident_clusters(const void* fn, int threads, size_t smem, int cluster, int* out);
+
 // Allow `fn` to use up to `smem` bytes of dynamic shared memory on the
 // current device (needed whenever static + dynamic exceeds 48 KB); cached per
 // (device, fn).
@@ -87,12 +92,12 @@ int per_launch_normalize(float* w, const int64_t* count, const float* gmax, int6
 // Operators of the learner. Arguments are checked by the entry points; NULL
 // pointers mean "absent" as described in per_b200.h.
 int per_launch_layer_norm(const per_norm_t& n, const void* x, int64_t x_stride, const void* weight,
-                          const void* bias, void* y, int64_t y_stride, double* mean, float* rstd,
+                          const void* bias, void* y, int64_t y_stride, float* stats,
                           cudaStream_t stream);
 int64_t per_layer_norm_backward_bytes(const per_norm_t& n);
 int per_launch_layer_norm_backward(const per_norm_t& n, const void* dy, int64_t dy_stride,
                                    const void* x, int64_t x_stride, const void* weight,
-                                   const double* mean, const float* rstd, void* dx,
+                                   const float* stats, void* dx,
                                    int64_t dx_stride, void* dweight, void* dbias, void* workspace,
                                    cudaStream_t stream);
 int64_t per_grad_norm_bytes(int64_t n);

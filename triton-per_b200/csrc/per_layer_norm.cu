@@ -9,8 +9,8 @@
 // s = fl(avg(x)), the sums of d = x - s and of d^2 give m = s + avg(d) and
 // v = avg(d^2) - avg(d)^2. s lies within rounding of the mean, so the
 // subtraction in v cancels nothing, and m is known to more than float32's
-// precision; it is kept as float64 and used as a pair of float32 (s, avg(d)),
-// because h loses |m| / sqrt(v) units of rounding to a mean held in float32.
+// precision; it is kept as the pair (s, avg(d)), because h loses
+// |m| / sqrt(v) units of rounding to a mean held in one float32.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -27,19 +27,18 @@ struct Fwd {
   const void* w;
   const void* b;
   void* y;
-  double* mean;
-  float* rstd;
+  float4* stats;  // mean as a sum of two, rstd, 0
   int64_t rows, x_stride, y_stride;
   int32_t dim;
   float eps;
+  int32_t group_threads;  // of a row that spans warps
 };
 
 struct Bwd {
   const void* dy;
   const void* x;
   const void* w;
-  const double* mean;
-  const float* rstd;
+  const float4* stats;
   void* dx;
   void* dw;
   void* db;
@@ -105,22 +104,19 @@ __device__ __forceinline__ void store(T* p, const Pack<T, VEC>& r) {
     *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(&r);
 }
 
-// The values of a thread, NV vectors of VEC, as pairs 0 .. NV VEC / 2. WORDS:
-// taken from and put into whole 32-bit words, which costs fewer instructions;
-// the forward kernel goes by single values, because from words the compiler
-// keeps weight and bias unpacked across rows and spills (65536x4096 bfloat16:
-// 178 us by values, 203 by words; backward 304 us by values, 290 by words).
-template <bool WORDS, typename T, int VEC, int NV>
+// The values of a thread, NV vectors of VEC, as pairs 0 .. NV VEC / 2, 16-bit
+// ones by whole words.
+template <typename T, int VEC, int NV>
 __device__ __forceinline__ float2 get2(const Pack<T, VEC> (&p)[NV], int i) {
-  if constexpr (WORDS && sizeof(T) == 2 && VEC > 1)
+  if constexpr (sizeof(T) == 2 && VEC > 1)
     return per_unpack<T>(reinterpret_cast<const uint32_t*>(&p[2 * i / VEC])[i % (VEC / 2)]);
   else
     return make_float2(per_to_f32(p[2 * i / VEC].v[2 * i % VEC]),
                        per_to_f32(p[(2 * i + 1) / VEC].v[(2 * i + 1) % VEC]));
 }
-template <bool WORDS, typename T, int VEC, int NV>
+template <typename T, int VEC, int NV>
 __device__ __forceinline__ void set2(Pack<T, VEC> (&p)[NV], int i, float2 f) {
-  if constexpr (WORDS && sizeof(T) == 2 && VEC > 1) {
+  if constexpr (sizeof(T) == 2 && VEC > 1) {
     reinterpret_cast<uint32_t*>(&p[2 * i / VEC])[i % (VEC / 2)] = per_pack<T>(f);
   } else {
     p[2 * i / VEC].v[2 * i % VEC] = per_from_f32<T>(f.x);
@@ -128,115 +124,160 @@ __device__ __forceinline__ void set2(Pack<T, VEC> (&p)[NV], int i, float2 f) {
   }
 }
 
-// The threads of a row: LANES of them (a power of two, several rows per
-// warp), a group of warps (LANES 0, one or several groups in a CTA), or a
-// cluster of CTAs (LANES -1, rows too long for one). Thread `lane` of `width`
-// holds the vectors lane, lane + width, ..., NV of them at most.
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t cluster_size() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return r;
-}
-
-template <int LANES>
-struct Row {
-  int lane, width;     // of this thread in its row
-  int64_t base, step;  // first row of this warp, rows between two of its turns
-  int mine;            // this thread's row is base + mine
-  int group;           // of this CTA's groups
-  int warps;           // of a row that spans warps
-  __device__ __forceinline__ explicit Row(int group_threads) {
-    mine = group = 0;
-    warps = 1;
-    if constexpr (LANES > 0) {
-      const int per_cta = blockDim.x / LANES;
-      lane = threadIdx.x % LANES;
-      width = LANES;
-      base = (int64_t)blockIdx.x * per_cta + (threadIdx.x & ~31) / LANES;
-      step = (int64_t)gridDim.x * per_cta;
-      mine = (threadIdx.x & 31) / LANES;
-    } else if constexpr (LANES == 0) {
-      const int groups = blockDim.x / group_threads;
-      group = threadIdx.x / group_threads;
-      lane = threadIdx.x - group * group_threads;
-      width = group_threads;
-      base = (int64_t)blockIdx.x * groups + group;
-      step = (int64_t)gridDim.x * groups;
-      warps = width >> 5;
-    } else {
-      const int ctas = (int)cluster_size();
-      lane = threadIdx.x + (int)(cluster_rank() * blockDim.x);
-      width = blockDim.x * ctas;
-      base = blockIdx.x / ctas;
-      step = gridDim.x / ctas;
-      warps = width >> 5;
-    }
-  }
-};
-
 template <int LANES>
 __device__ __forceinline__ float lanes_sum(float v) {
 #pragma unroll
-  for (int o = (LANES > 0 ? LANES : 32) / 2; o; o >>= 1) v += __shfl_xor_sync(PER_FULL_MASK, v, o);
+  for (int o = LANES / 2; o; o >>= 1) v += __shfl_xor_sync(PER_FULL_MASK, v, o);
   return v;
 }
 
-// What the warps of a row hand to one another: each warp's words go to every
-// CTA of the row, then one barrier. Two buffers by turns, so that one barrier
-// per exchange is enough: a buffer is written again only after the barrier of
-// the next exchange, which follows every read of it.
-constexpr int kMaxCluster = 8;
-constexpr int kRowThreads = 512;  // of a CTA whose warps share rows
+// The sums of a and of b over LANES lanes, in the time of one: a first step
+// leaves a to the even lanes and b to the odd ones. Even lanes return the sum
+// of a, odd lanes that of b.
 template <int LANES>
-struct Exchange {
-  float4 slot[2][LANES == 0 ? kRowThreads / 32 : kRowThreads / 32 * kMaxCluster];
-};
+__device__ __forceinline__ float lanes_sum_split(float a, float b) {
+  const bool odd = threadIdx.x & 1;
+  float v = odd ? b : a;
+  v += __shfl_xor_sync(PER_FULL_MASK, odd ? a : b, 1);
+#pragma unroll
+  for (int o = 2; o < LANES; o <<= 1) v += __shfl_xor_sync(PER_FULL_MASK, v, o);
+  return v;
+}
+// both sums in every lane, from what lanes_sum_split() returned
+__device__ __forceinline__ float2 join_split(float v) {
+  const float o = __shfl_xor_sync(PER_FULL_MASK, v, 1);
+  return (threadIdx.x & 1) ? make_float2(o, v) : make_float2(v, o);
+}
 
-template <int LANES>
-__device__ __forceinline__ void put(Exchange<LANES>& e, int turn, const Row<LANES>& t, float4 v) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if constexpr (LANES == 0) {
-    if (lane == 0) e.slot[turn][warp] = v;
-    __syncwarp();
-    asm volatile("bar.sync %0, %1;" ::"r"(t.group + 1), "r"(t.width) : "memory");
-  } else {
-    if (lane < (int)cluster_size()) {  // lane = the CTA that the warp's words go to
-      const float4* at = &e.slot[turn][cluster_rank() * (blockDim.x >> 5) + warp];
-      const uint32_t local = (uint32_t)__cvta_generic_to_shared(at);
-      uint32_t remote;
-      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(lane));
-      asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(remote), "f"(v.x),
-                   "f"(v.y), "f"(v.z), "f"(v.w)
-                   : "memory");
+// weight (or its absence as 1, bias as 0) of this thread's columns
+template <typename P, int VEC, int NV>
+__device__ __forceinline__ void load_columns(Pack<P, VEC> (&w)[NV], const void* p, float absent,
+                                             int first, int width, int dim) {
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = (first + k * width) * VEC;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) w[k].v[j] = per_from_f32<P>(absent);
+    if (c >= dim || !p) continue;
+    const P* q = static_cast<const P*>(p) + c;
+    if (VEC == 1 || (c + VEC <= dim && (uintptr_t)q % 16 == 0)) {
+      w[k] = load<P, VEC>(q);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        if (c + j < dim) w[k].v[j] = q[j];
     }
-    __syncwarp();
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
 }
 
-// The warps of a row as a lane sees them in an exchange: lane l reads warps
-// l mod span, + 32, ...; a butterfly over `span` lanes then joins them all.
-template <int LANES>
-struct Warps {
-  static constexpr int kReads = LANES == 0 ? 1 : kRowThreads / 32 * kMaxCluster / 32;
-  int span, first, from;
-  __device__ __forceinline__ explicit Warps(const Row<LANES>& t) {
-    span = 1;
-    while (span < t.warps && span < 32) span *= 2;
-    first = threadIdx.x & (span - 1);
-    from = LANES == 0 ? t.group * t.warps : 0;
+// Stops the compiler from holding 16-bit weights unpacked from row to row, in
+// twice the registers.
+template <typename P, int VEC, int NV>
+__device__ __forceinline__ void keep_packed(Pack<P, VEC> (&w)[NV]) {
+  if constexpr (sizeof(P) == 2 && VEC > 1) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int j = 0; j < VEC / 2; ++j)
+        asm volatile("" : "+r"(reinterpret_cast<uint32_t*>(&w[k])[j]));
   }
-  __device__ __forceinline__ float sum(float v) const {
-    for (int o = span >> 1; o; o >>= 1) v += __shfl_xor_sync(PER_FULL_MASK, v, o);
-    return v;
+}
+
+// v -= s in the row's columns; the values beyond them, read as 0, stay at 0.
+// The sums of v and of v^2.
+template <int VEC, int NV>
+__device__ __forceinline__ float2 centre(float2 (&v)[NV * VEC / 2], float s, int lane, int width,
+                                         int dim) {
+  const float2 m = per_both(-s);
+#pragma unroll
+  for (int i = 0; i < NV * VEC / 2; ++i) v[i] = per_add2(v[i], m);
+  if ((lane + (NV - 1) * width + 1) * VEC > dim) {  // the end of the row is among this thread's
+#pragma unroll
+    for (int i = 0; i < NV * VEC / 2; ++i) {
+      const int c0 = (lane + 2 * i / VEC * width) * VEC + 2 * i % VEC;
+      const int c1 = VEC > 1 ? c0 + 1 : lane + (2 * i + 1) * width;
+      if (c0 >= dim) v[i].x = 0.f;
+      if (c1 >= dim) v[i].y = 0.f;
+    }
   }
-};
+  float2 d1 = per_both(0.f), d2 = per_both(0.f);
+#pragma unroll
+  for (int i = 0; i < NV * VEC / 2; ++i) {
+    d1 = per_add2(d1, v[i]);
+    d2 = per_fma2(v[i], v[i], d2);
+  }
+  return make_float2(d1.x + d1.y, d2.x + d2.y);
+}
+
+// o = (v - shift) r w + b
+template <typename T, typename P, int VEC, int NV>
+__device__ __forceinline__ void normed(Pack<T, VEC> (&o)[NV], const float2 (&v)[NV * VEC / 2],
+                                       float shift, float r, const Pack<P, VEC> (&w)[NV],
+                                       const Pack<P, VEC> (&b)[NV]) {
+  const float2 r2 = per_both(r), c2 = per_both(-shift * r);
+#pragma unroll
+  for (int i = 0; i < NV * VEC / 2; ++i) set2(o, i, per_fma2(per_fma2(v[i], r2, c2), get2(w, i), get2(b, i)));
+}
+
+template <typename T, int VEC, int NV>
+__device__ __forceinline__ void store_row(T* y, const Pack<T, VEC> (&o)[NV], int lane, int width, int dim) {
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = (lane + k * width) * VEC;
+    if (c < dim) store<T, VEC>(y + c, o[k]);
+  }
+}
+
+// Backward sums of a row's values in a thread: h = (x - mean) r, g = dy w, the
+// column sums dw += dy h and db += dy, and the sums of g and of g h. Where
+// dy is 0 nothing is added.
+template <typename T, typename P, int VEC, int NV>
+__device__ __forceinline__ float2 backward_sums(const Pack<T, VEC> (&qx)[NV], const Pack<T, VEC> (&qy)[NV],
+                                                const Pack<P, VEC> (&w)[NV], float hi, float lo, float r,
+                                                float2 (&h)[NV * VEC / 2], float2 (&g)[NV * VEC / 2],
+                                                float2 (&aw)[NV * VEC / 2], float2 (&ab)[NV * VEC / 2]) {
+  const float2 m2 = per_both(-hi), r2 = per_both(r), lor = per_both(-lo * r);
+  float2 s1 = per_both(0.f), s2 = per_both(0.f);
+#pragma unroll
+  for (int i = 0; i < NV * VEC / 2; ++i) {
+    const float2 d = get2(qy, i);
+    h[i] = per_fma2(per_add2(get2(qx, i), m2), r2, lor);
+    aw[i] = per_fma2(d, h[i], aw[i]);
+    ab[i] = per_add2(ab[i], d);
+    g[i] = per_mul2(d, get2(w, i));
+    s1 = per_add2(s1, g[i]);
+    s2 = per_fma2(g[i], h[i], s2);
+  }
+  return make_float2(s1.x + s1.y, s2.x + s2.y);
+}
+
+// o = r (g - sum g / n - h sum(g h) / n)
+template <typename T, int VEC, int NV>
+__device__ __forceinline__ void backward_values(Pack<T, VEC> (&o)[NV], const float2 (&h)[NV * VEC / 2],
+                                                const float2 (&g)[NV * VEC / 2], float2 sums,
+                                                float inv_n, float r) {
+  const float2 r2 = per_both(r), k0 = per_both(-r * (sums.x * inv_n)),
+               k1 = per_both(-r * (sums.y * inv_n));
+#pragma unroll
+  for (int i = 0; i < NV * VEC / 2; ++i) set2(o, i, per_fma2(h[i], k1, per_fma2(g[i], r2, k0)));
+}
+
+// f(column of a value, dw, db) for a thread's column sums
+template <int VEC, int NV, typename F>
+__device__ __forceinline__ void for_columns(const float2 (&aw)[NV * VEC / 2],
+                                            const float2 (&ab)[NV * VEC / 2], int lane, int width,
+                                            int dim, F f) {
+#pragma unroll
+  for (int i = 0; i < NV * VEC / 2; ++i) {
+    const int c0 = (lane + 2 * i / VEC * width) * VEC + 2 * i % VEC;
+    const int c1 = VEC > 1 ? c0 + 1 : lane + (2 * i + 1) * width;
+    if (c0 < dim) f(c0, aw[i].x, ab[i].x);
+    if (c1 < dim) f(c1, aw[i].y, ab[i].y);
+  }
+}
+
+// ---- short rows: LANES threads of a warp (a power of two) per row, several
+// rows per warp, nothing but shuffles between the threads.
 
 // A thread's own copies on their way into shared memory, STAGES rows ahead:
 // it waits for and reads only what it has copied itself, so no barrier is
@@ -247,23 +288,25 @@ struct Ring {
   static constexpr bool kAsync = VEC * sizeof(T) == 16;
   static constexpr int kStages = kAsync ? STAGES : 1;
   static constexpr size_t kBytes = kAsync ? STAGES * NV * 16 : 0;  // per thread
+  const uint4* mine;
   uint32_t at;
   Pack<T, VEC> reg[kAsync ? 1 : NV];
 
   __device__ __forceinline__ explicit Ring(const void* smem) {
-    at = (uint32_t)__cvta_generic_to_shared(smem) + threadIdx.x * 16;
+    mine = static_cast<const uint4*>(smem) + threadIdx.x;
+    at = (uint32_t)__cvta_generic_to_shared(mine);
   }
-  // p is valid where `in` is true; base is always a valid address
-  __device__ __forceinline__ void fetch(int stage, int k, const T* base, int64_t offset, bool in) {
+  __device__ __forceinline__ void fetch(int stage, int k, const T* p, bool in) {
     if constexpr (kAsync) {
+      // a copy of 0 bytes reads nothing and fills the vector with zeros
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
                        at + (stage * NV + k) * blockDim.x * 16),
-                   "l"(in ? base + offset : base), "r"(in ? 16 : 0)
+                   "l"(p), "r"(in ? 16 : 0)
                    : "memory");
     } else {
 #pragma unroll
       for (int j = 0; j < VEC; ++j) reg[k].v[j] = per_from_f32<T>(0.f);
-      if (in) reg[k] = load<T, VEC>(base + offset);
+      if (in) reg[k] = load<T, VEC>(p);
     }
   }
   static __device__ __forceinline__ void commit() {
@@ -275,13 +318,8 @@ struct Ring {
   }
   __device__ __forceinline__ Pack<T, VEC> get(int stage, int k) {
     if constexpr (kAsync) {
-      uint4 u;
-      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
-                   : "r"(at + (stage * NV + k) * blockDim.x * 16)
-                   : "memory");
       Pack<T, VEC> r;
-      *reinterpret_cast<uint4*>(&r) = u;
+      *reinterpret_cast<uint4*>(&r) = mine[(stage * NV + k) * blockDim.x];
       return r;
     } else {
       return reg[k];
@@ -289,85 +327,37 @@ struct Ring {
   }
 };
 
-// Before a CTA writes into another one's shared memory, that one has to run.
-template <int LANES>
-__device__ __forceinline__ void cluster_begins() {
-  if constexpr (LANES < 0) {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-  }
-}
+constexpr int kWarpStages = 3;
 
-// weight (or its absence as 1, bias as 0) of this thread's columns
-template <typename P, int VEC, int NV>
-__device__ __forceinline__ void load_columns(Pack<P, VEC> (&w)[NV], const void* p, float absent,
-                                             int lane, int width, int dim) {
-#pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int c = (lane + k * width) * VEC;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) w[k].v[j] = per_from_f32<P>(absent);
-    if (c < dim && p) w[k] = load<P, VEC>(static_cast<const P*>(p) + c);
-  }
-}
-
-constexpr int kFwdStages = 3;
-constexpr int kBwdStages = 3;
-
-// ---- forward, rows in registers
 template <typename T, typename P, int VEC, int NV, int LANES>
-__global__ void __launch_bounds__(LANES > 0 ? 128 : kRowThreads) per_layer_norm_kernel(const Fwd f) {
-  __shared__ Exchange<LANES> ex;
+__global__ void __launch_bounds__(128) per_layer_norm_warp_kernel(const Fwd f) {
   extern __shared__ __align__(16) unsigned char dyn[];
-  const Row<LANES> t(blockDim.x);
-  using R = Ring<T, VEC, NV, kFwdStages>;
+  using R = Ring<T, VEC, NV, kWarpStages>;
   R ring(dyn);
-  int turn = 0, stage = 0;
-  constexpr int E2 = NV * VEC / 2;
+  int stage = 0;
+  const int lane = threadIdx.x % LANES, mine = (threadIdx.x & 31) / LANES;
+  const int per_cta = blockDim.x / LANES;
+  const int64_t step = (int64_t)gridDim.x * per_cta;
   const float n = (float)f.dim, inv_n = 1.f / n;
   const T* x = static_cast<const T*>(f.x);
-  T* y = static_cast<T*>(f.y);
-
-  // values of a warp (of a row that spans warps): this one's, and those of the
-  // warps that this lane reads in an exchange
-  const Warps<LANES> all(t);
-  auto values_of = [&](int warp) {
-    int v = 0;
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int left = f.dim / VEC - warp * 32 - k * t.width;
-      v += left < 0 ? 0 : left > 32 ? 32 : left;
-    }
-    return (float)(v * VEC);
-  };
-  constexpr int Q = Warps<LANES>::kReads;
-  float own = n, mq[Q];
-  if constexpr (LANES <= 0) {
-    own = values_of(t.lane >> 5);
-#pragma unroll
-    for (int i = 0; i < Q; ++i)
-      mq[i] = all.first + 32 * i < t.warps ? values_of(all.first + 32 * i) : 0.f;
-  }
-  const float inv_own = own > 0.f ? 1.f / own : 0.f;
-
-  cluster_begins<LANES>();
   per_wait_previous_grid();
   auto fetch = [&](int st, int64_t row) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int c = (t.lane + k * t.width) * VEC;
-      ring.fetch(st, k, x, row * f.x_stride + c, row < f.rows && c < f.dim);
+      const int c = (lane + k * LANES) * VEC;
+      ring.fetch(st, k, x + row * f.x_stride + c, row < f.rows && c < f.dim);
     }
     R::commit();
   };
+  int64_t base = (int64_t)blockIdx.x * per_cta + (threadIdx.x & ~31) / LANES;
 #pragma unroll
-  for (int k = 0; k < R::kStages; ++k) fetch(k, t.base + t.mine + k * t.step);
+  for (int k = 0; k < R::kStages; ++k) fetch(k, base + mine + k * step);
   Pack<P, VEC> w[NV], b[NV];
-  load_columns(w, f.w, 1.f, t.lane, t.width, f.dim);
-  load_columns(b, f.b, 0.f, t.lane, t.width, f.dim);
-  for (int64_t base = t.base; base < f.rows; base += t.step) {
-    const int64_t row = base + t.mine;
-    float2 v[E2];
+  load_columns(w, f.w, 1.f, lane, LANES, f.dim);
+  load_columns(b, f.b, 0.f, lane, LANES, f.dim);
+  for (; base < f.rows; base += step) {
+    const int64_t row = base + mine;
+    float2 v[NV * VEC / 2];
     float2 a = per_both(0.f);
     R::wait();
     {
@@ -375,132 +365,72 @@ __global__ void __launch_bounds__(LANES > 0 ? 128 : kRowThreads) per_layer_norm_
 #pragma unroll
       for (int k = 0; k < NV; ++k) q[k] = ring.get(stage, k);
 #pragma unroll
-      for (int i = 0; i < E2; ++i) {
-        v[i] = get2<false>(q, i);
+      for (int i = 0; i < NV * VEC / 2; ++i) {
+        v[i] = get2(q, i);
         a = per_add2(a, v[i]);
       }
     }
-    fetch(stage, row + R::kStages * t.step);
+    fetch(stage, row + R::kStages * step);
     stage = stage + 1 == R::kStages ? 0 : stage + 1;
-    // distances from a first mean: the row's, or (rows that span warps) the
-    // warp's; columns beyond the row, read as 0, stay at 0
-    const float s = over(lanes_sum<LANES>(a.x + a.y), own, inv_own);
-    float2 d1 = per_both(0.f), d2 = per_both(0.f);
-#pragma unroll
-    for (int i = 0; i < E2; ++i) {
-      const bool in0 = (t.lane + 2 * i / VEC * t.width) * VEC < f.dim;
-      const bool in1 = VEC > 1 ? in0 : (t.lane + (2 * i + 1) * t.width) < f.dim;
-      v[i] = per_add2(v[i], make_float2(in0 ? -s : 0.f, in1 ? -s : 0.f));
-      d1 = per_add2(d1, v[i]);
-      d2 = per_fma2(v[i], v[i], d2);
-    }
-    const float e1 = lanes_sum<LANES>(d1.x + d1.y);
-    const float e2 = lanes_sum<LANES>(d2.x + d2.y);
-    float shift, var;  // h = (v - shift) r
-    double mean;
-    if constexpr (LANES > 0) {
-      shift = over(e1, n, inv_n);
-      var = fmaf(-shift, shift, e2 * inv_n);
-      mean = (double)s + (double)shift;
-    } else {
-      // Warp q of m_q values: mean s_q + u_q with u_q = d1_q / m_q, squares around it
-      // d2_q - d1_q u_q. Seen from s_0 its mean lies at z_q; the row's at z = sum m_q z_q / n,
-      // and the row's squares are the warps' plus m_q (z_q - z)^2 each.
-      const float u = e1 * inv_own;
-      put<LANES>(ex, turn, t, make_float4(s, u, fmaxf(fmaf(-e1, u, e2), 0.f), 0.f));
-      const float s0 = ex.slot[turn][all.from].x;
-      float z = 0.f, sq = 0.f, zq[Q];
-#pragma unroll
-      for (int i = 0; i < Q; ++i) {
-        zq[i] = 0.f;
-        if (mq[i] > 0.f) {
-          const float4 o = ex.slot[turn][all.from + all.first + 32 * i];
-          zq[i] = (o.x - s0) + o.y;
-          sq += o.z;
-        }
-        z = fmaf(mq[i], zq[i], z);
-      }
-      turn ^= 1;
-      z = over(all.sum(z), n, inv_n);
-#pragma unroll
-      for (int i = 0; i < Q; ++i) sq = fmaf(mq[i] * (zq[i] - z), zq[i] - z, sq);
-      var = all.sum(sq) * inv_n;
-      shift = z - (s - s0);
-      mean = (double)s0 + (double)z;
-    }
+    const float s = over(lanes_sum<LANES>(a.x + a.y), n, inv_n);
+    const float2 e = centre<VEC, NV>(v, s, lane, LANES, f.dim);
+    const float shift = over(lanes_sum<LANES>(e.x), n, inv_n);
+    const float var = fmaf(-shift, shift, lanes_sum<LANES>(e.y) * inv_n);
     const float r = rsqrtf(fmaxf(var, 0.f) + f.eps);
-    const float2 r2 = per_both(r), c2 = per_both(-shift * r);
     if (row < f.rows) {
       Pack<T, VEC> o[NV];
-#pragma unroll
-      for (int i = 0; i < E2; ++i)
-        set2<false>(o, i, per_fma2(per_fma2(v[i], r2, c2), get2<false>(w, i), get2<false>(b, i)));
-#pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int c = (t.lane + k * t.width) * VEC;
-        if (c < f.dim) store<T, VEC>(y + row * f.y_stride + c, o[k]);
-      }
-      if (f.mean && t.lane == 0) {
-        f.mean[row] = mean;
-        f.rstd[row] = r;
-      }
+      normed<T, P, VEC, NV>(o, v, shift, r, w, b);
+      store_row(static_cast<T*>(f.y) + row * f.y_stride, o, lane, LANES, f.dim);
+      if (f.stats && lane == 0) f.stats[row] = make_float4(s, shift, r, 0.f);
     }
   }
 }
 
-// ---- backward, rows in registers: dx, and the column sums of this CTA's
-// rows. Each thread keeps the sums of its columns while its group walks down
-// the rows; at the end the groups of a CTA are joined in shared memory and
-// the CTA writes one partial row of dw and db. Columns beyond the row, and
-// rows beyond the last, read as dy = 0 and so add nothing to any sum.
+// Rows beyond the last read as dy = 0 and so add nothing to any sum.
 template <typename T, typename P, int VEC, int NV, int LANES>
-__global__ void __launch_bounds__(LANES > 0 ? 256 : kRowThreads)
-    per_layer_norm_backward_kernel(const Bwd g) {
-  __shared__ Exchange<LANES> ex;
+__global__ void __launch_bounds__(256) per_layer_norm_backward_warp_kernel(const Bwd g) {
   extern __shared__ __align__(16) unsigned char dyn[];
-  const Row<LANES> t(g.group_threads);
-  using R = Ring<T, VEC, 2 * NV, kBwdStages>;
+  using R = Ring<T, VEC, 2 * NV, kWarpStages>;
   R ring(dyn);
-  int turn = 0, stage = 0;
-  constexpr int E2 = NV * VEC / 2;
+  int stage = 0;
+  const int lane = threadIdx.x % LANES, mine = (threadIdx.x & 31) / LANES;
+  const int per_cta = blockDim.x / LANES;
+  const int64_t step = (int64_t)gridDim.x * per_cta;
   const float inv_n = 1.f / (float)g.dim;
-  const Warps<LANES> all(t);
   const T* x = static_cast<const T*>(g.x);
   const T* dy = static_cast<const T*>(g.dy);
-  T* dx = static_cast<T*>(g.dx);
-  cluster_begins<LANES>();
   per_wait_previous_grid();
   auto fetch = [&](int st, int64_t row) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int c = (t.lane + k * t.width) * VEC;
+      const int c = (lane + k * LANES) * VEC;
       const bool in = row < g.rows && c < g.dim;
-      ring.fetch(st, k, x, row * g.x_stride + c, in);
-      ring.fetch(st, NV + k, dy, row * g.dy_stride + c, in);
+      ring.fetch(st, k, x + row * g.x_stride + c, in);
+      ring.fetch(st, NV + k, dy + row * g.dy_stride + c, in);
     }
     R::commit();
   };
-  double nm = 0.0;
+  float2 nm = per_both(0.f);
   float nr = 0.f;
   auto fetch_stats = [&](int64_t row) {
     if (row >= g.rows) return;
-    nm = g.mean[row];
-    nr = g.rstd[row];
+    const float* st = reinterpret_cast<const float*>(g.stats + row);
+    nm = *reinterpret_cast<const float2*>(st);
+    nr = st[2];
   };
+  int64_t base = (int64_t)blockIdx.x * per_cta + (threadIdx.x & ~31) / LANES;
 #pragma unroll
-  for (int k = 0; k < R::kStages; ++k) fetch(k, t.base + t.mine + k * t.step);
-  fetch_stats(t.base + t.mine);
+  for (int k = 0; k < R::kStages; ++k) fetch(k, base + mine + k * step);
+  fetch_stats(base + mine);
   Pack<P, VEC> w[NV];
-  load_columns(w, g.w, 1.f, t.lane, t.width, g.dim);
-  float2 aw[E2], ab[E2];
+  load_columns(w, g.w, 1.f, lane, LANES, g.dim);
+  float2 aw[NV * VEC / 2], ab[NV * VEC / 2];
 #pragma unroll
-  for (int i = 0; i < E2; ++i) aw[i] = ab[i] = per_both(0.f);
-  for (int64_t base = t.base; base < g.rows; base += t.step) {
-    const int64_t row = base + t.mine;
-    const float hi = (float)nm, r = nr;
-    const float lo = (float)(nm - (double)hi);
-    float2 h[E2], gv[E2];
-    float2 s1 = per_both(0.f), s2 = per_both(0.f);
+  for (int i = 0; i < NV * VEC / 2; ++i) aw[i] = ab[i] = per_both(0.f);
+  for (; base < g.rows; base += step) {
+    const int64_t row = base + mine;
+    const float hi = nm.x, lo = nm.y, r = nr;
+    float2 h[NV * VEC / 2], gv[NV * VEC / 2], e;
     R::wait();
     {
       Pack<T, VEC> qx[NV], qy[NV];
@@ -509,86 +439,685 @@ __global__ void __launch_bounds__(LANES > 0 ? 256 : kRowThreads)
         qx[k] = ring.get(stage, k);
         qy[k] = ring.get(stage, NV + k);
       }
-#pragma unroll
-      for (int i = 0; i < E2; ++i) {
-        const float2 d = get2<true>(qy, i);
-        h[i] = per_fma2(per_add2(get2<true>(qx, i), per_both(-hi)), per_both(r), per_both(-lo * r));
-        aw[i] = per_fma2(d, h[i], aw[i]);
-        ab[i] = per_add2(ab[i], d);
-        gv[i] = per_mul2(d, get2<true>(w, i));
-        s1 = per_add2(s1, gv[i]);
-        s2 = per_fma2(gv[i], h[i], s2);
-      }
+      e = backward_sums(qx, qy, w, hi, lo, r, h, gv, aw, ab);
     }
-    fetch(stage, row + R::kStages * t.step);
-    fetch_stats(row + t.step);
+    fetch(stage, row + R::kStages * step);
+    fetch_stats(row + step);
     stage = stage + 1 == R::kStages ? 0 : stage + 1;
     if (!g.dx) continue;
-    float a = lanes_sum<LANES>(s1.x + s1.y), q = lanes_sum<LANES>(s2.x + s2.y);
-    if constexpr (LANES <= 0) {
-      put<LANES>(ex, turn, t, make_float4(a, q, 0.f, 0.f));
-      a = q = 0.f;
-#pragma unroll
-      for (int i = 0; i < Warps<LANES>::kReads; ++i)
-        if (all.first + 32 * i < t.warps) {
-          const float4 o = ex.slot[turn][all.from + all.first + 32 * i];
-          a += o.x;
-          q += o.y;
-        }
-      turn ^= 1;
-      a = all.sum(a);
-      q = all.sum(q);
-    }
+    const float2 sums = join_split(lanes_sum_split<LANES>(e.x, e.y));
     if (row < g.rows) {
-      // r (g - a / n - h q / n)
-      const float2 r2 = per_both(r), k0 = per_both(-r * (a * inv_n)), k1 = per_both(-r * (q * inv_n));
       Pack<T, VEC> o[NV];
-#pragma unroll
-      for (int i = 0; i < E2; ++i) set2<true>(o, i, per_fma2(h[i], k1, per_fma2(gv[i], r2, k0)));
-#pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int c = (t.lane + k * t.width) * VEC;
-        if (c < g.dim) store<T, VEC>(dx + row * g.dx_stride + c, o[k]);
-      }
+      backward_values<T, VEC, NV>(o, h, gv, sums, inv_n, r);
+      store_row(static_cast<T*>(g.dx) + row * g.dx_stride, o, lane, LANES, g.dim);
     }
   }
   if (!g.part) return;
-  if (LANES < 0 || (LANES == 0 && t.width == (int)blockDim.x)) {
-    float* part = g.part + t.base * 2 * g.dim;
+  // the row groups of a warp by shuffles, then the warps through shared
+  // memory, where the (empty) copies still in flight have ended
+  float* part = g.part + (int64_t)blockIdx.x * 2 * g.dim;
+  float* sums = reinterpret_cast<float*>(dyn);  // [warps][2][dim]
+  float* own = sums + (threadIdx.x >> 5) * 2 * g.dim;
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();
 #pragma unroll
-    for (int i = 0; i < E2; ++i) {
-      const int c0 = (t.lane + 2 * i / VEC * t.width) * VEC + 2 * i % VEC;
-      const int c1 = VEC > 1 ? c0 + 1 : t.lane + (2 * i + 1) * t.width;
-      if (c0 < g.dim) part[c0] = aw[i].x, part[g.dim + c0] = ab[i].x;
-      if (c1 < g.dim) part[c1] = aw[i].y, part[g.dim + c1] = ab[i].y;
+  for (int i = 0; i < NV * VEC / 2; ++i)
+#pragma unroll
+    for (int o = LANES; o < 32; o <<= 1) {
+      aw[i].x += __shfl_xor_sync(PER_FULL_MASK, aw[i].x, o);
+      aw[i].y += __shfl_xor_sync(PER_FULL_MASK, aw[i].y, o);
+      ab[i].x += __shfl_xor_sync(PER_FULL_MASK, ab[i].x, o);
+      ab[i].y += __shfl_xor_sync(PER_FULL_MASK, ab[i].y, o);
     }
-  } else if constexpr (LANES >= 0) {
-    // the row groups of a warp by shuffles, then the groups through shared
-    // memory, where the (empty) copies still in flight have ended
-    float* part = g.part + (int64_t)blockIdx.x * 2 * g.dim;
-    float* sums = reinterpret_cast<float*>(dyn);  // [groups][2][dim]
-    const int group = LANES > 0 ? threadIdx.x >> 5 : t.group;
-    const int groups = LANES > 0 ? blockDim.x >> 5 : blockDim.x / t.width;
-    float* mine = sums + group * 2 * g.dim;
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < E2; ++i) {
-      if constexpr (LANES > 0) {
-#pragma unroll
-        for (int o = LANES; o < 32; o <<= 1) {
-          aw[i].x += __shfl_xor_sync(PER_FULL_MASK, aw[i].x, o);
-          aw[i].y += __shfl_xor_sync(PER_FULL_MASK, aw[i].y, o);
-          ab[i].x += __shfl_xor_sync(PER_FULL_MASK, ab[i].x, o);
-          ab[i].y += __shfl_xor_sync(PER_FULL_MASK, ab[i].y, o);
-        }
+  if (mine == 0)
+    for_columns<VEC, NV>(aw, ab, lane, LANES, g.dim, [&](int c, float dw, float db) {
+      own[c] = dw;
+      own[g.dim + c] = db;
+    });
+  __syncthreads();
+  for (int c = threadIdx.x; c < 2 * g.dim; c += blockDim.x) {
+    float v = 0.f;
+    for (int q = 0; q < (int)(blockDim.x >> 5); ++q) v += sums[q * 2 * g.dim + c];
+    part[c] = v;
+  }
+}
+
+// ---- longer rows: a group of warps per row (several groups in a CTA), or a
+// cluster of CTAs per row, each with a slice of it.
+
+constexpr int kMaxCluster = 8;
+constexpr int kRowThreads = 512;  // of a CTA
+constexpr int kMaxGroups = 8;
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// A thread's place: `lane` of `width` threads that hold the values first ..
+// first + dim of a row.
+template <bool CLUSTER>
+struct Group {
+  int lane, width, index;  // index: of this CTA's groups
+  int first, dim;          // this CTA's slice of the row
+  int warps;               // of all CTAs of the row
+  int64_t base, step;      // first row, rows between two turns
+  __device__ __forceinline__ Group(int threads, int vec, int nv, int row_dim) {
+    const int groups = CLUSTER ? 1 : blockDim.x / threads;
+    index = CLUSTER ? 0 : threadIdx.x / threads;
+    lane = threadIdx.x - index * threads;
+    width = threads;
+    first = 0;
+    dim = row_dim;
+    warps = width >> 5;
+    base = (int64_t)blockIdx.x * groups + index;
+    step = (int64_t)gridDim.x * groups;
+    if constexpr (CLUSTER) {
+      const int ctas = (int)cluster_size();
+      base = blockIdx.x / ctas;
+      step = gridDim.x / ctas;
+      warps *= ctas;
+      const int slice = threads * nv * vec;
+      first = (int)cluster_rank() * slice;
+      dim = row_dim - first;
+      dim = dim < 0 ? 0 : dim > slice ? slice : dim;
+    }
+  }
+};
+
+// What the warps of a row hand to one another. In one CTA: each warp's words,
+// then a barrier of the group. Over a cluster: each warp's words go to every
+// CTA by st.async, which counts their bytes on a barrier word there that the
+// CTA's threads wait for; a cluster barrier in its place also waits for the
+// output rows that the threads have stored before.
+// Two buffers by turns, so that one barrier per exchange is enough: a buffer is
+// written again only in the next exchange but one, whose sender has waited for
+// the exchange between, and with it for all readers of this one.
+template <bool CLUSTER>
+struct Exchange {
+  static constexpr int kWarps = kRowThreads / 32 * (CLUSTER ? kMaxCluster : 1);
+  float4 slot[2][kWarps];
+  uint64_t arrived[2];  // CLUSTER
+};
+
+__device__ __forceinline__ uint32_t remote_address(const void* p, uint32_t cta) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+               : "=r"(r)
+               : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(cta));
+  return r;
+}
+
+// The state of a thread in the exchanges of its row.
+template <bool CLUSTER>
+struct Turns {
+  int turn = 0, parity = 0;
+  bool failed = false;  // a wait has given up: nothing that follows is waited for
+  // Once, by all threads of the CTA; a cluster barrier has to follow.
+  __device__ __forceinline__ void begin(Exchange<CLUSTER>& e) {
+    if constexpr (CLUSTER)
+      if (threadIdx.x == 0) {
+        per_mbar_init(&e.arrived[0], 1);
+        per_mbar_init(&e.arrived[1], 1);
+        per_fence_mbar_init();
       }
-      const int c0 = (t.lane + 2 * i / VEC * t.width) * VEC + 2 * i % VEC;
-      const int c1 = VEC > 1 ? c0 + 1 : t.lane + (2 * i + 1) * t.width;
-      if (t.mine == 0 && c0 < g.dim) mine[c0] = aw[i].x, mine[g.dim + c0] = ab[i].x;
-      if (t.mine == 0 && c1 < g.dim) mine[c1] = aw[i].y, mine[g.dim + c1] = ab[i].y;
+  }
+  // The words that each warp sends (`bytes` of them) are here.
+  __device__ __forceinline__ void wait(Exchange<CLUSTER>& e, int warps, int bytes) {
+    if constexpr (CLUSTER) {
+      if (threadIdx.x == 0 && !failed) per_mbar_arrive_expect_tx(&e.arrived[turn], warps * bytes);
+      if (!failed) failed = !per_mbar_wait(&e.arrived[turn], parity, nullptr);
     }
+  }
+  __device__ __forceinline__ void next() {
+    turn ^= 1;
+    parity ^= turn ^ 1;  // flips when both buffers have had their turn
+  }
+};
+
+// Among the threads of one CTA that share a row.
+template <bool CLUSTER>
+__device__ __forceinline__ void cta_part_sync(const Group<CLUSTER>& t) {
+  __syncwarp();
+  if (t.width > 32) asm volatile("bar.sync %0, %1;" ::"r"(t.index + 1), "r"(t.width) : "memory");
+}
+template <bool CLUSTER>
+__device__ __forceinline__ void put(Exchange<CLUSTER>& e, Turns<CLUSTER>& turns, const Group<CLUSTER>& t,
+                                    float4 v) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if constexpr (!CLUSTER) {
+    if (lane == 0) e.slot[turns.turn][warp] = v;
+    cta_part_sync(t);
+  } else {
+    if (lane < (int)cluster_size()) {  // lane = the CTA that the warp's words go to
+      const uint32_t to =
+          remote_address(&e.slot[turns.turn][cluster_rank() * (blockDim.x >> 5) + warp], lane);
+      asm volatile(
+          "st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to),
+          "r"(__float_as_uint(v.x)), "r"(__float_as_uint(v.y)), "r"(__float_as_uint(v.z)),
+          "r"(__float_as_uint(v.w)), "r"(remote_address(&e.arrived[turns.turn], lane))
+          : "memory");
+    }
+    turns.wait(e, t.warps, 16);
+  }
+}
+
+// The warps of a row as a lane sees them in an exchange: lane l reads warps
+// l mod span, + 32, ...; a butterfly over `span` lanes then joins them all.
+template <bool CLUSTER>
+struct Warps {
+  static constexpr int kReads = Exchange<CLUSTER>::kWarps > 32 ? Exchange<CLUSTER>::kWarps / 32 : 1;
+  int span, first, from;
+  __device__ __forceinline__ explicit Warps(const Group<CLUSTER>& t) {
+    span = 1;
+    while (span < t.warps && span < 32) span *= 2;
+    first = threadIdx.x & (span - 1);
+    from = t.index * t.warps;
+  }
+  __device__ __forceinline__ float sum(float v) const {
+    for (int o = span >> 1; o; o >>= 1) v += __shfl_xor_sync(PER_FULL_MASK, v, o);
+    return v;
+  }
+};
+
+// lanes_sum_split() of a warp in, that of the whole row out. `span`: lanes'
+// worth of warps, a power of two up to 16.
+template <bool CLUSTER>
+__device__ __forceinline__ float exchange_split(Exchange<CLUSTER>& e, Turns<CLUSTER>& turns,
+                                                const Group<CLUSTER>& t, int span, float v) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float* slots = reinterpret_cast<float*>(e.slot[turns.turn]);  // [warp][2]
+  if constexpr (!CLUSTER) {
+    if (lane < 2) slots[2 * warp + lane] = v;
+    cta_part_sync(t);
+  } else {
+    if (lane < 2 * (int)cluster_size()) {  // lanes 2 c and 2 c + 1: to CTA c
+      const uint32_t to = remote_address(
+          &slots[2 * (cluster_rank() * (blockDim.x >> 5) + warp) + (lane & 1)], lane >> 1);
+      asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(to),
+                   "r"(__float_as_uint(v)), "r"(remote_address(&e.arrived[turns.turn], lane >> 1))
+                   : "memory");
+    }
+    turns.wait(e, t.warps, 8);
+  }
+  turns.next();
+  const int first = 2 * t.index * t.warps, at = lane & (2 * span - 1);
+  v = 0.f;
+#pragma unroll
+  for (int i = 0; i < (CLUSTER ? Exchange<CLUSTER>::kWarps / 16 : 1); ++i)
+    if (at + 32 * i < 2 * t.warps) v += slots[first + at + 32 * i];
+  for (int o = span; o > 1; o >>= 1) v += __shfl_xor_sync(PER_FULL_MASK, v, o);
+  return v;
+}
+
+// One of the arrays whose rows a kernel reads: this CTA's slice of row r is the
+// `dim` values from first + r stride on. [begin, end): what the rows of the
+// array span.
+template <typename T>
+struct Array {
+  const T* first;
+  int64_t stride;
+  uintptr_t begin, end;
+  __device__ __forceinline__ Array(const void* p, int64_t row_stride, int64_t rows, int row_dim,
+                                   int slice_first)
+      : first(static_cast<const T*>(p) + slice_first), stride(row_stride) {
+    begin = (uintptr_t)p;
+    end = begin + (uintptr_t)((rows - 1) * row_stride + row_dim) * sizeof(T);
+  }
+  __device__ __forceinline__ const T* row(int64_t r) const { return first + r * stride; }
+  // where row r starts between two 16-byte boundaries
+  __device__ __forceinline__ int phase(int64_t r) const {
+    return (int)(((uint32_t)(uintptr_t)first + (uint32_t)r * (uint32_t)(stride * (int64_t)sizeof(T))) & 15u);
+  }
+};
+
+// 16 bytes from any element boundary of shared memory: vector i past `phase`
+// bytes (0 .. 15) from a 16-byte boundary.
+__device__ __forceinline__ uint4 window(const unsigned char* base, int i, int phase) {
+  const uint4* p = reinterpret_cast<const uint4*>(base) + i;
+  const uint4 a = p[0], b = p[1];
+  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  if (phase & 8)
+#pragma unroll
+    for (int j = 0; j < 6; ++j) w[j] = w[j + 2];
+  if (phase & 4)
+#pragma unroll
+    for (int j = 0; j < 5; ++j) w[j] = w[j + 1];
+  const int shift = (phase & 3) * 8;
+  return make_uint4(__funnelshift_r(w[0], w[1], shift), __funnelshift_r(w[1], w[2], shift),
+                    __funnelshift_r(w[2], w[3], shift), __funnelshift_r(w[3], w[4], shift));
+}
+
+// The rows of a group on their way into shared memory, STAGES of them, ARRAYS
+// arrays each (plus, STATS, the 16 bytes of a row's statistics), by bulk copies
+// that one thread issues, so that the others spend no instruction on
+// addresses. A slot is filled again once a barrier of the group has followed
+// its reading.
+//
+// ANY false: rows are whole vectors on 16-byte boundaries. ANY: rows of any
+// length that start anywhere; the copy takes the 16-byte blocks that hold a row
+// (its neighbours' values come along and are masked), except where such a block
+// would reach beyond the array, before its first row or behind its last: those
+// rows are fetched value by value.
+template <typename T, int NV, int ARRAYS, int STAGES, bool STATS, bool ANY>
+struct Rows {
+  static constexpr int VEC = 16 / sizeof(T);
+  unsigned char* slots;
+  uint64_t* bars;
+  int array_bytes, slot_bytes;
+  int stage, parity;
+  bool failed;  // a wait has given up: nothing that follows is waited for
+  int phase[ARRAYS];
+
+  // shared memory of one array's slice (ANY: a vector more than the slice, for
+  // the phase, and one that window() reads), and of a group
+  static __host__ __device__ int room(int width) { return width * NV * 16 + (ANY ? 32 : 0); }
+  static __host__ __device__ size_t bytes(int width) {
+    return (size_t)STAGES * (ARRAYS * room(width) + 16);
+  }
+  __device__ __forceinline__ Rows(unsigned char* smem, uint64_t* group_bars, int width) {
+    slots = smem;
+    bars = group_bars;
+    array_bytes = room(width);
+    slot_bytes = ARRAYS * array_bytes + 16;
+    stage = parity = 0;
+    failed = false;
+#pragma unroll
+    for (int a = 0; a < ARRAYS; ++a) phase[a] = 0;
+  }
+  // Once, before anything else, by all threads of the group: the barriers, and
+  // zeros for the vectors beyond the slice, which no copy writes (ANY: get()
+  // masks them). A barrier of the CTA has to follow.
+  __device__ __forceinline__ void begin(int dim, int lane, int width) {
+    if (lane == 0) {
+      for (int k = 0; k < STAGES; ++k) per_mbar_init(bars + k, 1);
+      per_fence_mbar_init();
+    }
+    if constexpr (!ANY) {
+      for (int k = 0; k < STAGES * ARRAYS; ++k) {
+        unsigned char* array = slots + k / ARRAYS * slot_bytes + k % ARRAYS * array_bytes;
+        for (int i = dim * (int)sizeof(T) + lane * 16; i < array_bytes; i += width * 16)
+          *reinterpret_cast<uint4*>(array + i) = make_uint4(0, 0, 0, 0);
+      }
+      per_fence_proxy_async_smem();
+    }
+  }
+  // Fill slot `st` with row r (`in`: there is one). All threads of the group
+  // call it.
+  __device__ __forceinline__ void fetch(int st, const Array<T> (&arrays)[ARRAYS], const float4* stats,
+                                        int64_t r, int dim, int lane, int width, bool in) {
+    if (!in || failed) return;
+    unsigned char* slot = slots + st * slot_bytes;
+    if constexpr (!ANY) {
+      if (lane) return;
+      const uint32_t bytes = (uint32_t)dim * sizeof(T);
+      per_mbar_arrive_expect_tx(bars + st, ARRAYS * bytes + (STATS ? 16 : 0));
+#pragma unroll
+      for (int a = 0; a < ARRAYS; ++a)
+        if (bytes) per_bulk_load(slot + a * array_bytes, arrays[a].row(r), bytes, bars + st);
+    } else {
+      uint32_t bytes[ARRAYS], all = STATS ? 16 : 0;
+      uintptr_t from[ARRAYS];
+#pragma unroll
+      for (int a = 0; a < ARRAYS; ++a) {
+        const T* p = arrays[a].row(r);
+        from[a] = (uintptr_t)p & ~(uintptr_t)15;
+        const uintptr_t to = ((uintptr_t)(p + dim) + 15) & ~(uintptr_t)15;
+        bytes[a] = dim ? (uint32_t)(to - from[a]) : 0;
+        if (dim && (from[a] < arrays[a].begin || to > arrays[a].end)) {
+          bytes[a] = 0;  // value by value
+          T* out = reinterpret_cast<T*>(slot + a * array_bytes + ((uintptr_t)p & 15));
+          for (int c = lane; c < dim; c += width) out[c] = p[c];
+          per_fence_proxy_async_smem();  // before a later copy into the same slot
+        }
+        all += bytes[a];
+      }
+      if (lane) return;
+      per_mbar_arrive_expect_tx(bars + st, all);
+#pragma unroll
+      for (int a = 0; a < ARRAYS; ++a)
+        if (bytes[a])
+          per_bulk_load(slot + a * array_bytes, reinterpret_cast<const void*>(from[a]), bytes[a],
+                        bars + st);
+    }
+    if (STATS) per_bulk_load(slot + ARRAYS * array_bytes, stats + r, 16, bars + st);
+  }
+  // Wait for row r, the next one.
+  __device__ __forceinline__ void wait(const Array<T> (&arrays)[ARRAYS], int64_t r) {
+    if (!failed) failed = !per_mbar_wait(bars + stage, parity, nullptr);
+    if constexpr (ANY)
+#pragma unroll
+      for (int a = 0; a < ARRAYS; ++a) phase[a] = arrays[a].phase(r);
+  }
+  // Vector `lane + k width` of the row's slice, zeros beyond its end.
+  __device__ __forceinline__ Pack<T, VEC> get(int a, int k, int dim, int lane, int width) const {
+    const unsigned char* array = slots + stage * slot_bytes + a * array_bytes;
+    const int i = lane + k * width;
+    Pack<T, VEC> q;
+    if constexpr (!ANY) {
+      *reinterpret_cast<uint4*>(&q) = *reinterpret_cast<const uint4*>(array + i * 16);
+    } else {
+      *reinterpret_cast<uint4*>(&q) = window(array, i, phase[a]);
+      if ((i + 1) * VEC > dim) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          if (i * VEC + j >= dim) q.v[j] = per_from_f32<T>(0.f);
+      }
+    }
+    return q;
+  }
+  __device__ __forceinline__ float4 get_stats() const {
+    return *reinterpret_cast<const float4*>(slots + stage * slot_bytes + ARRAYS * array_bytes);
+  }
+  __device__ __forceinline__ void next() {
+    if (++stage == STAGES) {
+      stage = 0;
+      parity ^= 1;
+    }
+  }
+  // After the last row. Where a wait gave up, copies may still be on their way
+  // into this CTA's memory: wait once more for each, within the same limit.
+  __device__ __forceinline__ void end() {
+    if (failed)
+      for (int k = 0; k < STAGES; ++k)
+        per_mbar_wait(bars + k, k < stage ? parity ^ 1 : parity, nullptr);
+  }
+};
+
+// The way out for rows of any length that start anywhere: each thread puts its
+// vectors into shared memory and takes those back that lie on 16-byte
+// boundaries of the output; values at either end are stored one by one.
+template <typename T, int NV>
+struct Outbox {
+  static constexpr int VEC = 16 / sizeof(T);
+  static __host__ __device__ size_t bytes(int width) { return (size_t)width * NV * 16 + 48; }
+
+  // Between two barriers of the group, of which the second is its own.
+  template <bool CLUSTER>
+  static __device__ __forceinline__ void store_row(unsigned char* box, T* y, const Pack<T, VEC> (&o)[NV],
+                                                   const Group<CLUSTER>& t) {
+    // the row begins one vector into the box
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      *reinterpret_cast<uint4*>(box + 16 + (t.lane + k * t.width) * 16) =
+          *reinterpret_cast<const uint4*>(&o[k]);
+    cta_part_sync(t);
+    const int phase = (int)((uintptr_t)y & 15), first = -phase / (int)sizeof(T);
+    unsigned char* out = reinterpret_cast<unsigned char*>(y) - phase;  // on a boundary
+    const int skip = (16 - phase) >> 4;  // 1 where the row begins on one
+#pragma unroll
+    for (int k = 0; k <= NV; ++k) {
+      const int i = t.lane + k * t.width;
+      const int c = first + i * VEC;  // of the block's first value
+      if (c >= t.dim || (k == NV && t.lane > 0)) continue;
+      Pack<T, VEC> q;
+      *reinterpret_cast<uint4*>(&q) = window(box, i + skip, (16 - phase) & 15);
+      if (c >= 0 && c + VEC <= t.dim) {
+        *reinterpret_cast<uint4*>(out + (int64_t)i * 16) = *reinterpret_cast<const uint4*>(&q);
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          if (c + j >= 0 && c + j < t.dim) y[c + j] = q.v[j];
+      }
+    }
+  }
+};
+
+// The forward kernel takes bulk copies where rows start anywhere or spread over
+// a cluster; whole vectors of rows in one CTA come by the threads' own cp.async
+// copies, which need no wait on a barrier and were as fast or faster
+// (32768x4096 bfloat16, float32 weights: 92 us against 115; bfloat16 weights:
+// 88 and 88; 32768x2048: 54 and 61).
+template <bool CLUSTER, bool ANY>
+constexpr bool kFwdBulk = ANY || CLUSTER;
+constexpr int kFwdStages = 3;
+// Threads that a CTA is compiled for, which bounds a thread's registers. 32
+// values of 16-bit rows with their weights and biases take some 144: CTAs of
+// up to 192 threads get them (168 each, and as many CTAs per SM), since what
+// the compiler spills at 128 costs up to half the time (32768x4096 bfloat16:
+// 88 us without, 100 to 140 with). Larger CTAs keep 16-bit weights packed
+// instead (16384x8192: 140 -> 104 us).
+template <typename T, int NV>
+constexpr bool kWide = sizeof(T) == 2 && NV == 4;
+constexpr int kWideThreads = 384;
+// Three rows ahead; two where an outbox has to fit beside them.
+template <bool ANY>
+constexpr int kBwdStages = ANY ? 2 : 3;
+
+template <typename T, typename P, int NV, bool CLUSTER, bool ANY, int THREADS>
+__global__ void __launch_bounds__(THREADS) per_layer_norm_group_kernel(const Fwd f) {
+  __shared__ Exchange<CLUSTER> ex;
+  __shared__ __align__(8) uint64_t bars[kMaxGroups][kFwdStages];
+  extern __shared__ __align__(16) unsigned char dyn[];
+  constexpr int VEC = 16 / sizeof(T);
+  constexpr bool kBulk = kFwdBulk<CLUSTER, ANY>;
+  using R = Rows<T, NV, 1, kFwdStages, false, ANY>;
+  using C = Ring<T, VEC, NV, kFwdStages>;
+  const Group<CLUSTER> t(f.group_threads, VEC, NV, f.dim);
+  unsigned char* mine = dyn + t.index * (R::bytes(t.width) + (ANY ? Outbox<T, NV>::bytes(t.width) : 0));
+  R rows(mine, bars[t.index], t.width);
+  C ring(dyn);
+  if constexpr (kBulk) rows.begin(t.dim, t.lane, t.width);
+  Turns<CLUSTER> turns;
+  turns.begin(ex);
+  int stage = 0;
+  const float n = (float)f.dim, inv_n = 1.f / n;
+  const Array<T> x[1] = {Array<T>(f.x, f.x_stride, f.rows, f.dim, t.first)};
+  T* y = static_cast<T*>(f.y) + t.first;
+
+  // values of a warp of the row: this one's, and those of the warps that this
+  // lane reads in an exchange
+  const Warps<CLUSTER> all(t);
+  auto values_of = [&](int warp) {
+    const int per_cta = t.width >> 5, rank = CLUSTER ? warp / per_cta : 0;
+    const int dim = f.dim - rank * t.width * NV * VEC;  // from that CTA's slice on
+    int v = 0;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int left = dim - ((warp - rank * per_cta) * 32 + k * t.width) * VEC;
+      v += left < 0 ? 0 : left > 32 * VEC ? 32 * VEC : left;
+    }
+    return (float)v;
+  };
+  constexpr int Q = Warps<CLUSTER>::kReads;
+  float mq[Q];
+  const float own = values_of((t.lane >> 5) + (CLUSTER ? (int)cluster_rank() * (t.width >> 5) : 0));
+#pragma unroll
+  for (int i = 0; i < Q; ++i)
+    mq[i] = all.first + 32 * i < t.warps ? values_of(all.first + 32 * i) : 0.f;
+  const float inv_own = own > 0.f ? 1.f / own : 0.f;
+
+  if constexpr (CLUSTER)
+    cluster_sync();  // before a CTA writes into another one's shared memory, that one has to run
+  else
     __syncthreads();
+  per_wait_previous_grid();
+  auto fetch = [&](int st, int64_t row) {
+    if constexpr (kBulk) {
+      rows.fetch(st, x, nullptr, row, t.dim, t.lane, t.width, row < f.rows);
+    } else {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int c = (t.lane + k * t.width) * VEC;
+        ring.fetch(st, k, x[0].row(row) + c, row < f.rows && c < t.dim);
+      }
+      C::commit();
+    }
+  };
+  for (int k = 0; k < kFwdStages; ++k) fetch(k, t.base + k * t.step);
+  if constexpr (ANY) cta_part_sync(t);  // values that were fetched one by one
+  Pack<P, VEC> w[NV], b[NV];
+  load_columns(w, f.w ? static_cast<const P*>(f.w) + t.first : nullptr, 1.f, t.lane, t.width, t.dim);
+  load_columns(b, f.b ? static_cast<const P*>(f.b) + t.first : nullptr, 0.f, t.lane, t.width, t.dim);
+  for (int64_t row = t.base; row < f.rows; row += t.step) {
+    float2 v[NV * VEC / 2];
+    float2 a = per_both(0.f);
+    if constexpr (kWide<T, NV> && THREADS > kWideThreads) {
+      keep_packed(w);
+      keep_packed(b);
+    }
+    if constexpr (kBulk)
+      rows.wait(x, row);
+    else
+      C::wait();
+    {
+      Pack<T, VEC> q[NV];
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+        if constexpr (kBulk)
+          q[k] = rows.get(0, k, t.dim, t.lane, t.width);
+        else
+          q[k] = ring.get(stage, k);
+#pragma unroll
+      for (int i = 0; i < NV * VEC / 2; ++i) {
+        v[i] = get2(q, i);
+        a = per_add2(a, v[i]);
+      }
+    }
+    if constexpr (!kBulk) {
+      fetch(stage, row + kFwdStages * t.step);
+      stage = stage + 1 == kFwdStages ? 0 : stage + 1;
+    }
+    // Distances from the warp's own mean first. Warp q of m_q values then has the mean
+    // s_q + u_q with u_q = d1_q / m_q, and squares around it d2_q - d1_q u_q. Seen from s_0 its
+    // mean lies at z_q; the row's at z = sum m_q z_q / n, and the row's squares are the warps'
+    // plus m_q (z_q - z)^2 each.
+    const float s = over(lanes_sum<32>(a.x + a.y), own, inv_own);
+    const float2 e = centre<VEC, NV>(v, s, t.lane, t.width, t.dim);
+    const float e1 = lanes_sum<32>(e.x), e2 = lanes_sum<32>(e.y);
+    const float u = e1 * inv_own;
+    put(ex, turns, t, make_float4(s, u, fmaxf(fmaf(-e1, u, e2), 0.f), 0.f));
+    if constexpr (kBulk) fetch(rows.stage, row + kFwdStages * t.step);
+    const float s0 = ex.slot[turns.turn][all.from].x;
+    float z = 0.f, sq = 0.f, zq[Q];
+#pragma unroll
+    for (int i = 0; i < Q; ++i) {
+      zq[i] = 0.f;
+      if (mq[i] > 0.f) {
+        const float4 o = ex.slot[turns.turn][all.from + all.first + 32 * i];
+        zq[i] = (o.x - s0) + o.y;
+        sq += o.z;
+      }
+      z = fmaf(mq[i], zq[i], z);
+    }
+    turns.next();
+    z = over(all.sum(z), n, inv_n);
+#pragma unroll
+    for (int i = 0; i < Q; ++i) sq = fmaf(mq[i] * (zq[i] - z), zq[i] - z, sq);
+    const float var = all.sum(sq) * inv_n;
+    float r = rsqrtf(fmaxf(var, 0.f) + f.eps);
+    if ((kBulk && rows.failed) || turns.failed) r = __int_as_float(0x7fc00000);  // something never came: say so in the result
+    Pack<T, VEC> o[NV];
+    normed<T, P, VEC, NV>(o, v, z - (s - s0), r, w, b);
+    if constexpr (ANY)
+      Outbox<T, NV>::store_row(mine + R::bytes(t.width), y + row * f.y_stride, o, t);
+    else
+      store_row(y + row * f.y_stride, o, t.lane, t.width, t.dim);
+    if (f.stats && t.lane == 0 && t.first == 0) f.stats[row] = make_float4(s0, z, r, 0.f);
+    if constexpr (kBulk) rows.next();
+  }
+  if constexpr (kBulk) rows.end();
+  if constexpr (CLUSTER) cluster_sync();  // no CTA ends while another may still write to it
+}
+
+// dx, and the column sums of this CTA's rows: each thread keeps the sums of
+// its columns while its group walks down the rows; at the end the groups of a
+// CTA are joined in shared memory and the CTA writes one partial row of dw and
+// db. Columns beyond the row read as dy = 0 and so add nothing to any sum.
+template <typename T, typename P, int NV, bool CLUSTER, bool ANY>
+__global__ void __launch_bounds__(kRowThreads) per_layer_norm_backward_group_kernel(const Bwd g) {
+  constexpr int VEC = 16 / sizeof(T), kStages = kBwdStages<ANY>;
+  __shared__ Exchange<CLUSTER> ex;
+  __shared__ __align__(8) uint64_t bars[kMaxGroups][kStages];
+  extern __shared__ __align__(16) unsigned char dyn[];
+  using R = Rows<T, NV, 2, kStages, true, ANY>;
+  using O = Outbox<T, NV>;
+  const Group<CLUSTER> t(g.group_threads, VEC, NV, g.dim);
+  unsigned char* own = dyn + t.index * (R::bytes(t.width) + (ANY ? O::bytes(t.width) : 0));
+  R rows(own, bars[t.index], t.width);
+  rows.begin(t.dim, t.lane, t.width);
+  Turns<CLUSTER> turns;
+  turns.begin(ex);
+  const float inv_n = 1.f / (float)g.dim;
+  int span = 1;
+  while (span < t.warps && span < 16) span *= 2;
+  const Array<T> in[2] = {Array<T>(g.x, g.x_stride, g.rows, g.dim, t.first),
+                          Array<T>(g.dy, g.dy_stride, g.rows, g.dim, t.first)};
+  T* dx = static_cast<T*>(g.dx) + t.first;
+  if constexpr (CLUSTER)
+    cluster_sync();
+  else
+    __syncthreads();
+  per_wait_previous_grid();
+  auto fetch = [&](int st, int64_t row) {
+    rows.fetch(st, in, g.stats, row, t.dim, t.lane, t.width, row < g.rows);
+  };
+  for (int k = 0; k < kStages; ++k) fetch(k, t.base + k * t.step);
+  if constexpr (ANY) cta_part_sync(t);  // values that were fetched one by one
+  Pack<P, VEC> w[NV];
+  load_columns(w, g.w ? static_cast<const P*>(g.w) + t.first : nullptr, 1.f, t.lane, t.width, t.dim);
+  float2 aw[NV * VEC / 2], ab[NV * VEC / 2];
+#pragma unroll
+  for (int i = 0; i < NV * VEC / 2; ++i) aw[i] = ab[i] = per_both(0.f);
+  for (int64_t row = t.base; row < g.rows; row += t.step) {
+    float2 h[NV * VEC / 2], gv[NV * VEC / 2], e;
+    rows.wait(in, row);
+    const float4 st = rows.get_stats();
+    const bool failed = rows.failed || turns.failed;
+    const float r = failed ? __int_as_float(0x7fc00000) : st.z;  // NaN: something never came
+    {
+      Pack<T, VEC> qx[NV], qy[NV];
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        qx[k] = rows.get(0, k, t.dim, t.lane, t.width);
+        qy[k] = rows.get(1, k, t.dim, t.lane, t.width);
+      }
+      e = backward_sums(qx, qy, w, st.x, st.y, r, h, gv, aw, ab);
+    }
+    const float v = exchange_split(ex, turns, t, span, lanes_sum_split<32>(e.x, e.y));
+    fetch(rows.stage, row + kStages * t.step);
+    if (g.dx) {
+      Pack<T, VEC> o[NV];
+      backward_values<T, VEC, NV>(o, h, gv, join_split(v), inv_n,
+                                  turns.failed ? __int_as_float(0x7fc00000) : r);
+      if constexpr (ANY)
+        O::store_row(own + R::bytes(t.width), dx + row * g.dx_stride, o, t);
+      else
+        store_row(dx + row * g.dx_stride, o, t.lane, t.width, t.dim);
+    }
+    rows.next();
+  }
+  rows.end();
+  if constexpr (CLUSTER) cluster_sync();  // no CTA ends while another may still write to it
+  if (!g.part) return;
+  if (CLUSTER || t.width == (int)blockDim.x) {
+    float* part = g.part + t.base * 2 * g.dim + t.first;
+    for_columns<VEC, NV>(aw, ab, t.lane, t.width, t.dim, [&](int c, float dw, float db) {
+      part[c] = dw;
+      part[g.dim + c] = db;
+    });
+  } else {
+    float* part = g.part + (int64_t)blockIdx.x * 2 * g.dim;
+    float* sums = reinterpret_cast<float*>(dyn);  // [groups][2][dim], over the slots, all of them read
+    float* mine = sums + t.index * 2 * g.dim;
+    __syncthreads();
+    for_columns<VEC, NV>(aw, ab, t.lane, t.width, t.dim, [&](int c, float dw, float db) {
+      mine[c] = dw;
+      mine[g.dim + c] = db;
+    });
+    __syncthreads();
+    const int groups = blockDim.x / t.width;
     for (int c = threadIdx.x; c < 2 * g.dim; c += blockDim.x) {
       float v = 0.f;
       for (int q = 0; q < groups; ++q) v += sums[q * 2 * g.dim + c];
@@ -626,10 +1155,7 @@ __global__ void __launch_bounds__(kThreads) per_layer_norm_long_kernel(const Fwd
       if (b) h += per_to_f32(b[c]);
       y[c] = per_from_f32<T>(h);
     }
-    if (f.mean && threadIdx.x == 0) {
-      f.mean[row] = (double)s + (double)shift;
-      f.rstd[row] = r;
-    }
+    if (f.stats && threadIdx.x == 0) f.stats[row] = make_float4(s, shift, r, 0.f);
   }
 }
 
@@ -642,8 +1168,8 @@ __global__ void __launch_bounds__(kThreads) per_layer_norm_dx_long_kernel(const 
     const T* x = static_cast<const T*>(g.x) + row * g.x_stride;
     const T* dy = static_cast<const T*>(g.dy) + row * g.dy_stride;
     T* dx = static_cast<T*>(g.dx) + row * g.dx_stride;
-    const double m = g.mean[row];
-    const float hi = (float)m, lo = (float)(m - (double)hi), r = g.rstd[row];
+    const float4 st = g.stats[row];
+    const float hi = st.x, lo = st.y, r = st.z;
     float a = 0.f, q = 0.f;
     for (int64_t c = threadIdx.x; c < g.dim; c += kThreads) {
       const float h = (per_to_f32(x[c]) - hi - lo) * r;
@@ -673,8 +1199,8 @@ __global__ void __launch_bounds__(kThreads) per_layer_norm_dw_long_kernel(const 
   const T* dy = static_cast<const T*>(g.dy) + c;
   float dw = 0.f, db = 0.f;
   for (int64_t row = split; row < g.rows; row += g.splits) {
-    const double m = g.mean[row];
-    const float hi = (float)m, lo = (float)(m - (double)hi), r = g.rstd[row];
+    const float4 st = g.stats[row];
+    const float hi = st.x, lo = st.y, r = st.z;
     const float v = per_to_f32(dy[row * g.dy_stride]);
     dw = fmaf(v, (per_to_f32(x[row * g.x_stride]) - hi - lo) * r, dw);
     db += v;
@@ -739,9 +1265,9 @@ int splits_of(int64_t rows, int64_t dim) {
   return s < 1 ? 1 : (int)s;
 }
 
-// How a row is laid over threads: `lanes` of a warp with `nv` vectors each, or
-// a group of `threads` of each of `ctas` CTAs (lanes 0). ctas 0: too long for
-// registers.
+// How a row is laid over threads: `lanes` of a warp, or a group of `threads`
+// in each of `ctas` CTAs (lanes 0), with `nv` vectors per thread. ctas 0: too
+// long for registers.
 struct Shape {
   int lanes, nv, threads, ctas;
 };
@@ -749,47 +1275,60 @@ struct Shape {
 // Most vectors of a row that a thread holds. The sums over a row cost a thread
 // some 100 instructions whatever it holds, so it should hold much; statistics,
 // weights and (backward) two column sums per value have to fit its registers.
-template <typename T, int VEC>
-constexpr int fwd_vectors() {
-  return VEC == 1 ? 16 : 4;
-}
-template <typename T, int VEC>
-constexpr int bwd_vectors() {
-  return VEC == 1 ? 8 : sizeof(T) == 2 ? 2 : 4;
-}
+constexpr int kFwdVectors = 4;
+template <typename T>
+constexpr int kBwdVectors = sizeof(T) == 2 ? 2 : 4;
+constexpr int kSingles = 8;  // of single values, in a warp
 
 // Rows that a warp can hold stay in it, which needs no barrier; longer ones
-// take a group of warps, and beyond one CTA a cluster of up to 8.
-Shape shape_of(int64_t dim, int vec, int full, int warp_threads) {
-  const int64_t v = (dim + vec - 1) / vec;
-  const int small = vec == 1 ? 4 : 1;
+// take a group of warps, and beyond one CTA a cluster of up to 8. In a warp,
+// rows that start anywhere go by single values (vec 1).
+Shape shape_of(int64_t dim, int vec, bool any, bool split, int full, int most_threads,
+               int warp_threads) {
+  const int small = any ? 4 : 1, most = any ? kSingles : full;
+  const int64_t w = any ? dim : (dim + vec - 1) / vec;
   for (int lanes = 4; lanes <= 32; lanes *= 2)
-    if (v <= lanes * small) return {lanes, small, warp_threads, 1};
-  for (int nv = 2 * small; nv <= full; nv *= 2)
-    if (v <= 32 * nv) return {32, nv, warp_threads, 1};
-  for (int ctas = 1; ctas <= kMaxCluster; ctas *= 2)
-    if (v <= (int64_t)ctas * kRowThreads * full) {
-      const int64_t threads = (v + ctas * full - 1) / (ctas * full);
-      return {0, full, (int)((threads + 31) / 32 * 32), ctas};
-    }
-  return {0, 0, 0, 0};
+    if (w <= lanes * small) return {lanes, small, warp_threads, 1};
+  for (int nv = 2 * small; nv <= most; nv *= 2)
+    if (w <= 32 * nv) return {32, nv, warp_threads, 1};
+  const int64_t v = (dim + vec - 1) / vec;
+  int ctas = 1;
+  while (v > (int64_t)ctas * most_threads * full)
+    if ((ctas *= 2) > kMaxCluster) return {0, 0, 0, 0};
+  const auto threads = [&](int nv) { return (v + ctas * nv * 32 - 1) / (ctas * nv * 32) * 32; };
+  // An SM has registers for some 512 threads: CTAs of more than 256 leave some of
+  // them idle. Twice the CTAs then (20001 bfloat16 values, backward: 195 -> 162
+  // us; 10000 float32 ones, forward: 148 -> 122 us), except in the backward pass
+  // of whole vectors, where the wider cluster costs more (10000 float32 values:
+  // 153 -> 179 us).
+  while (split && threads(full) > 256 && threads(full) < (any ? kRowThreads + 1 : 448) &&
+         ctas < kMaxCluster)
+    ctas *= 2;
+  // as many vectors a thread as there may be, or half, where that leaves fewer places empty
+  const int nv = threads(full / 2) <= most_threads && 8 * threads(full / 2) <= 13 * threads(full)
+                     ? full / 2 : full;
+  return {0, nv, (int)threads(nv), ctas};
 }
 
-// go<T, P, VEC, NV, LANES>(shape, ...) for the shape into rc; false where
-// there is none
-#define PER_NORM_SHAPE(s, rc, go, T, P, VEC, FULL, ...)                                        \
+// warp<T, P, VEC, NV, LANES>(...) or group<T, P, NV, CLUSTER, ANY>(...) for the
+// shape, into rc; false where there is none
+#define PER_NORM_SHAPE(s, rc, warp, group, T, P, ANY, FULL, ...)                               \
   [&]() -> bool {                                                                              \
-    constexpr int S = VEC == 1 ? 4 : 1, F = FULL;                                              \
-    if (s.lanes == 4) return rc = go<T, P, VEC, S, 4>(s, __VA_ARGS__), true;                   \
-    if (s.lanes == 8) return rc = go<T, P, VEC, S, 8>(s, __VA_ARGS__), true;                   \
-    if (s.lanes == 16) return rc = go<T, P, VEC, S, 16>(s, __VA_ARGS__), true;                 \
-    if (s.lanes == 32 && s.nv == S) return rc = go<T, P, VEC, S, 32>(s, __VA_ARGS__), true;    \
+    constexpr int V = ANY ? 1 : 16 / sizeof(T), S = ANY ? 4 : 1, F = FULL;                     \
+    constexpr int W = ANY ? kSingles : F;                                                      \
+    if (s.lanes == 4) return rc = warp<T, P, V, S, 4>(s, __VA_ARGS__), true;                   \
+    if (s.lanes == 8) return rc = warp<T, P, V, S, 8>(s, __VA_ARGS__), true;                   \
+    if (s.lanes == 16) return rc = warp<T, P, V, S, 16>(s, __VA_ARGS__), true;                 \
+    if (s.lanes == 32 && s.nv == S) return rc = warp<T, P, V, S, 32>(s, __VA_ARGS__), true;    \
     if (s.lanes == 32 && s.nv == 2 * S)                                                        \
-      return rc = go<T, P, VEC, 2 * S, 32>(s, __VA_ARGS__), true;                              \
-    if constexpr (F >= 4 * S)                                                                  \
-      if (s.lanes == 32) return rc = go<T, P, VEC, 4 * S, 32>(s, __VA_ARGS__), true;           \
-    if (s.ctas == 1) return rc = go<T, P, VEC, F, 0>(s, __VA_ARGS__), true;                    \
-    if (s.ctas > 1) return rc = go<T, P, VEC, F, -1>(s, __VA_ARGS__), true;                    \
+      return rc = warp<T, P, V, 2 * S, 32>(s, __VA_ARGS__), true;                              \
+    if constexpr (W >= 4 * S)                                                                  \
+      if (s.lanes == 32) return rc = warp<T, P, V, 4 * S, 32>(s, __VA_ARGS__), true;           \
+    if (s.ctas == 1 && s.nv == F)                                                              \
+      return rc = group<T, P, F, false, ANY>(s, __VA_ARGS__), true;                            \
+    if (s.ctas == 1) return rc = group<T, P, F / 2, false, ANY>(s, __VA_ARGS__), true;         \
+    if (s.ctas > 1 && s.nv == F) return rc = group<T, P, F, true, ANY>(s, __VA_ARGS__), true;  \
+    if (s.ctas > 1) return rc = group<T, P, F / 2, true, ANY>(s, __VA_ARGS__), true;           \
     return false;                                                                              \
   }()
 
@@ -803,44 +1342,60 @@ int row_ctas(const void* fn, const Shape& s, int threads, size_t smem, int64_t r
   int rc = per_set_smem(fn, smem);
   if (rc) return rc;
   int ctas = 0;
-  rc = per_coresident_ctas(fn, threads, smem, &ctas);
+  rc = per_coresident_clusters(fn, threads, smem, s.ctas, &ctas);
   if (rc) return rc;
   const int64_t per_cta = threads / (s.lanes ? s.lanes : s.threads);
   int64_t grid = (rows - 1) / per_cta + 1;
-  const int64_t room = ctas / s.ctas > 0 ? ctas / s.ctas : 1;
-  if (grid > room) grid = room;
+  if (grid > ctas) grid = ctas;
   if (most > 0 && grid > most) grid = most;
   *out = grid;
   return PER_OK;
 }
 
 template <typename T, typename P, int VEC, int NV, int LANES>
-int forward_go(const Shape& s, const Fwd& f, cudaStream_t stream) {
-  const void* fn = (const void*)per_layer_norm_kernel<T, P, VEC, NV, LANES>;
-  const size_t smem = Ring<T, VEC, NV, kFwdStages>::kBytes * s.threads;
+int forward_warp(const Shape& s, const Fwd& f, cudaStream_t stream) {
+  const void* fn = (const void*)per_layer_norm_warp_kernel<T, P, VEC, NV, LANES>;
+  const size_t smem = Ring<T, VEC, NV, kWarpStages>::kBytes * s.threads;
   int64_t grid = 0;
   const int rc = row_ctas(fn, s, s.threads, smem, f.rows, 0, &grid);
-  if (rc) return rc;
-  return launch(fn, grid * s.ctas, s.threads, smem, &f, stream, s.ctas);
+  return rc ? rc : launch(fn, grid, s.threads, smem, &f, stream);
 }
 
-template <typename T, typename P, int VEC>
-int forward_vec(const Fwd& f, cudaStream_t stream) {
-  constexpr int FULL = fwd_vectors<T, VEC>();
-  const Shape s = shape_of(f.dim, VEC, FULL, 128);
+template <typename T, typename P, int NV, bool CLUSTER, bool ANY>
+int forward_group(const Shape& s, const Fwd& in, cudaStream_t stream) {
+  Fwd f = in;
+  f.group_threads = s.threads;
+  const void* fn = (const void*)per_layer_norm_group_kernel<T, P, NV, CLUSTER, ANY, kRowThreads>;
+  if constexpr (kWide<T, NV>)
+    if (s.threads <= 192)
+      fn = (const void*)per_layer_norm_group_kernel<T, P, NV, CLUSTER, ANY, kWideThreads>;
+  // rows of few threads share a CTA of about 128
+  const int groups = CLUSTER || !ANY || s.threads > 64 ? 1 : 128 / s.threads;
+  const size_t smem = kFwdBulk<CLUSTER, ANY>
+                          ? groups * (Rows<T, NV, 1, kFwdStages, false, ANY>::bytes(s.threads) +
+                                      (ANY ? Outbox<T, NV>::bytes(s.threads) : 0))
+                          : Ring<T, 16 / sizeof(T), NV, kFwdStages>::kBytes * s.threads;
+  int64_t grid = 0;
+  const int rc = row_ctas(fn, s, s.threads * groups, smem, f.rows, 0, &grid);
+  return rc ? rc : launch(fn, grid * s.ctas, s.threads * groups, smem, &f, stream, s.ctas);
+}
+
+template <typename T, typename P, bool ANY>
+int forward_rows(const Fwd& f, cudaStream_t stream) {
+  constexpr int FULL = kFwdVectors;
+  const Shape s = shape_of(f.dim, 16 / sizeof(T), ANY, true, FULL, kRowThreads, 128);
   int rc = PER_OK;
-  if (PER_NORM_SHAPE(s, rc, forward_go, T, P, VEC, FULL, f, stream)) return rc;
+  if (PER_NORM_SHAPE(s, rc, forward_warp, forward_group, T, P, ANY, FULL, f, stream)) return rc;
   return launch((const void*)per_layer_norm_long_kernel<T, P>, row_grid(f.rows), kThreads, 0, &f,
                 stream);
 }
 
 template <typename T, typename P>
 int forward(const Fwd& f, cudaStream_t stream) {
-  constexpr int VEC = 16 / sizeof(T);
-  if (f.dim % VEC == 0 && aligned(f.x, f.x_stride, sizeof(T)) &&
+  if (f.dim % (16 / sizeof(T)) == 0 && aligned(f.x, f.x_stride, sizeof(T)) &&
       aligned(f.y, f.y_stride, sizeof(T)) && aligned(f.w, 0, 1) && aligned(f.b, 0, 1))
-    return forward_vec<T, P, VEC>(f, stream);
-  return forward_vec<T, P, 1>(f, stream);
+    return forward_rows<T, P, false>(f, stream);
+  return forward_rows<T, P, true>(f, stream);
 }
 
 // Most partial rows of dw and db (the workspace is sized before the pointers'
@@ -850,19 +1405,9 @@ int64_t most_partials(int64_t rows, int64_t dim) {
   return rows < most ? rows : most;
 }
 
-template <typename T, typename P, int VEC, int NV, int LANES>
-int backward_go(const Shape& s, const Bwd& in, cudaStream_t stream) {
-  Bwd g = in;
-  const void* fn = (const void*)per_layer_norm_backward_kernel<T, P, VEC, NV, LANES>;
-  // a CTA of about 256 threads: several groups share its partial row
-  const int groups = LANES == 0 && s.threads <= 128 ? 256 / s.threads : 1;
-  const int threads = s.threads * groups;
-  g.group_threads = s.threads;
-  size_t smem = Ring<T, VEC, 2 * NV, kBwdStages>::kBytes * threads;
-  if (LANES > 0 || groups > 1) {
-    const size_t sums = (size_t)(LANES > 0 ? threads / 32 : groups) * 2 * g.dim * 4;
-    smem = smem > sums ? smem : sums;
-  }
+// The row kernel, then the join of its partial rows where columns are wanted.
+template <typename P>
+int backward_run(const void* fn, const Shape& s, int threads, size_t smem, Bwd g, cudaStream_t stream) {
   int64_t grid = 0;
   int rc = row_ctas(fn, s, threads, smem, g.rows, most_partials(g.rows, g.dim), &grid);
   if (rc) return rc;
@@ -875,12 +1420,35 @@ int backward_go(const Shape& s, const Bwd& in, cudaStream_t stream) {
                 kJoinThreads, 0, &g, stream);
 }
 
-template <typename T, typename P, int VEC>
-int backward_vec(const Bwd& in, cudaStream_t stream) {
-  constexpr int FULL = bwd_vectors<T, VEC>();
-  const Shape s = shape_of(in.dim, VEC, FULL, 256);
+template <typename T, typename P, int VEC, int NV, int LANES>
+int backward_warp(const Shape& s, const Bwd& g, cudaStream_t stream) {
+  const size_t ring = Ring<T, VEC, 2 * NV, kWarpStages>::kBytes * s.threads;
+  const size_t sums = (size_t)(s.threads / 32) * 2 * g.dim * 4;
+  return backward_run<P>((const void*)per_layer_norm_backward_warp_kernel<T, P, VEC, NV, LANES>, s,
+                         s.threads, ring > sums ? ring : sums, g, stream);
+}
+
+template <typename T, typename P, int NV, bool CLUSTER, bool ANY>
+int backward_group(const Shape& s, const Bwd& in, cudaStream_t stream) {
+  Bwd g = in;
+  g.group_threads = s.threads;
+  // several groups share a CTA and its partial row
+  int groups = CLUSTER ? 1 : kRowThreads / s.threads;
+  groups = groups > kMaxGroups ? kMaxGroups : groups;
+  size_t smem = groups * (Rows<T, NV, 2, kBwdStages<ANY>, true, ANY>::bytes(s.threads) +
+                          (ANY ? Outbox<T, NV>::bytes(s.threads) : 0));
+  const size_t sums = groups > 1 ? (size_t)groups * 2 * g.dim * 4 : 0;
+  smem = smem > sums ? smem : sums;
+  return backward_run<P>((const void*)per_layer_norm_backward_group_kernel<T, P, NV, CLUSTER, ANY>, s,
+                         s.threads * groups, smem, g, stream);
+}
+
+template <typename T, typename P, bool ANY>
+int backward_rows(const Bwd& in, cudaStream_t stream) {
+  constexpr int FULL = kBwdVectors<T>;
+  const Shape s = shape_of(in.dim, 16 / sizeof(T), ANY, ANY, FULL, kRowThreads, 256);
   int rc = PER_OK;
-  if (PER_NORM_SHAPE(s, rc, backward_go, T, P, VEC, FULL, in, stream)) return rc;
+  if (PER_NORM_SHAPE(s, rc, backward_warp, backward_group, T, P, ANY, FULL, in, stream)) return rc;
   Bwd g = in;
   g.splits = splits_of(g.rows, g.dim);
   if (g.dx)
@@ -897,12 +1465,11 @@ int backward_vec(const Bwd& in, cudaStream_t stream) {
 
 template <typename T, typename P>
 int backward(const Bwd& g, cudaStream_t stream) {
-  constexpr int VEC = 16 / sizeof(T);
-  if (g.dim % VEC == 0 && aligned(g.x, g.x_stride, sizeof(T)) &&
+  if (g.dim % (16 / sizeof(T)) == 0 && aligned(g.x, g.x_stride, sizeof(T)) &&
       aligned(g.dy, g.dy_stride, sizeof(T)) && aligned(g.dx, g.dx_stride, sizeof(T)) &&
       aligned(g.w, 0, 1))
-    return backward_vec<T, P, VEC>(g, stream);
-  return backward_vec<T, P, 1>(g, stream);
+    return backward_rows<T, P, false>(g, stream);
+  return backward_rows<T, P, true>(g, stream);
 }
 
 }  // namespace
@@ -917,9 +1484,9 @@ int backward(const Bwd& g, cudaStream_t stream) {
                                 : fn<__half, __half>(__VA_ARGS__))
 
 int per_launch_layer_norm(const per_norm_t& n, const void* x, int64_t x_stride, const void* weight,
-                          const void* bias, void* y, int64_t y_stride, double* mean, float* rstd,
+                          const void* bias, void* y, int64_t y_stride, float* stats,
                           cudaStream_t stream) {
-  const Fwd f{x, weight, bias, y, mean, rstd, n.rows, x_stride, y_stride, (int32_t)n.dim, n.eps};
+  const Fwd f{x, weight, bias, y, reinterpret_cast<float4*>(stats), n.rows, x_stride, y_stride, (int32_t)n.dim, n.eps, 0};
   return PER_NORM_TYPES(n, forward, f, stream);
 }
 
@@ -932,10 +1499,11 @@ int64_t per_layer_norm_backward_bytes(const per_norm_t& n) {
 
 int per_launch_layer_norm_backward(const per_norm_t& n, const void* dy, int64_t dy_stride,
                                    const void* x, int64_t x_stride, const void* weight,
-                                   const double* mean, const float* rstd, void* dx,
+                                   const float* stats, void* dx,
                                    int64_t dx_stride, void* dweight, void* dbias, void* workspace,
                                    cudaStream_t stream) {
-  const Bwd g{dy, x, weight, mean, rstd, dx, dweight, dbias, static_cast<float*>(workspace),
+  const Bwd g{dy, x, weight, reinterpret_cast<const float4*>(stats), dx, dweight, dbias,
+              static_cast<float*>(workspace),
               n.rows, dy_stride, x_stride, dx_stride, (int32_t)n.dim, 0, 0};
   return PER_NORM_TYPES(n, backward, g, stream);
 }

@@ -74,21 +74,20 @@ int check_norm_call(const per_tensor_t* t, int64_t n, int32_t kind, const float*
 extern "C" {
 
 int per_layer_norm(const per_norm_t* norm, const void* x, int64_t x_stride, const void* weight,
-                   const void* bias, void* y, int64_t y_stride, double* mean, float* rstd,
-                   void* stream) {
+                   const void* bias, void* y, int64_t y_stride, float* stats, void* stream) {
   PerRange range("per_layer_norm");
   const int rc = check_norm(norm);
   if (rc) return rc;
   if (!(norm->eps >= 0.f)) return PER_ERR_INVALID_ARGUMENT;
   if (norm->rows == 0) return PER_OK;
-  if (!x || !y || (!mean) != (!rstd)) return PER_ERR_NULL_POINTER;
+  if (!x || !y) return PER_ERR_NULL_POINTER;
   if (x_stride < norm->dim || y_stride < norm->dim) return PER_ERR_INVALID_ARGUMENT;
   const int64_t eb = per_dtype_bytes(norm->dtype), pb = per_dtype_bytes(norm->param_dtype);
   if (misaligned(x, eb) || misaligned(y, eb) || misaligned(weight, pb) || misaligned(bias, pb) ||
-      misaligned(mean, 8) || misaligned(rstd, 4))
+      misaligned(stats, 16))
     return PER_ERR_MISALIGNED;
   if (rows_overlap(norm, x, x_stride, y, y_stride)) return PER_ERR_INVALID_ARGUMENT;
-  return per_launch_layer_norm(*norm, x, x_stride, weight, bias, y, y_stride, mean, rstd,
+  return per_launch_layer_norm(*norm, x, x_stride, weight, bias, y, y_stride, stats,
                                (cudaStream_t)stream);
 }
 
@@ -99,17 +98,16 @@ int64_t per_layer_norm_backward_workspace(const per_norm_t* norm) {
 
 int per_layer_norm_backward(const per_norm_t* norm, const void* dy, int64_t dy_stride,
                             const void* x, int64_t x_stride, const void* weight,
-                            const double* mean, const float* rstd, void* dx, int64_t dx_stride,
-                            void* dweight, void* dbias, void* workspace, int64_t workspace_bytes,
-                            void* stream) {
+                            const float* stats, void* dx, int64_t dx_stride, void* dweight,
+                            void* dbias, void* workspace, int64_t workspace_bytes, void* stream) {
   PerRange range("per_layer_norm_backward");
   const int rc = check_norm(norm);
   if (rc) return rc;
   if (!dx && !dweight && !dbias) return PER_OK;
   const int64_t eb = per_dtype_bytes(norm->dtype), pb = per_dtype_bytes(norm->param_dtype);
   if (misaligned(dweight, pb) || misaligned(dbias, pb) || misaligned(weight, pb) ||
-      misaligned(dy, eb) || misaligned(x, eb) || misaligned(dx, eb) || misaligned(mean, 8) ||
-      misaligned(rstd, 4) || misaligned(workspace, 16))
+      misaligned(dy, eb) || misaligned(x, eb) || misaligned(dx, eb) || misaligned(stats, 16) ||
+       misaligned(workspace, 16))
     return PER_ERR_MISALIGNED;
   const cudaStream_t s = (cudaStream_t)stream;
   if (norm->rows == 0) {
@@ -121,7 +119,7 @@ int per_layer_norm_backward(const per_norm_t* norm, const void* dy, int64_t dy_s
     }
     return PER_OK;
   }
-  if (!dy || !x || !mean || !rstd) return PER_ERR_NULL_POINTER;
+  if (!dy || !x || !stats) return PER_ERR_NULL_POINTER;
   if ((dy_stride != 0 && dy_stride < norm->dim) || x_stride < norm->dim ||
       (dx && dx_stride < norm->dim))
     return PER_ERR_INVALID_ARGUMENT;
@@ -131,7 +129,7 @@ int per_layer_norm_backward(const per_norm_t* norm, const void* dy, int64_t dy_s
   if (dx && (rows_overlap(norm, x, x_stride, dx, dx_stride) ||
              rows_overlap(norm, dy, dy_stride, dx, dx_stride)))
     return PER_ERR_INVALID_ARGUMENT;
-  return per_launch_layer_norm_backward(*norm, dy, dy_stride, x, x_stride, weight, mean, rstd, dx,
+  return per_launch_layer_norm_backward(*norm, dy, dy_stride, x, x_stride, weight, stats, dx,
                                         dx_stride, dweight, dbias, workspace, s);
 }
 

@@ -94,7 +94,7 @@ struct Shape {
 
 struct LayerNormBackward : public torch::autograd::Node {
   torch::autograd::SavedVariable x, weight;
-  Tensor mean, rstd;
+  Tensor stats;
   bool has_weight = false, has_bias = false;
   at::ScalarType param_type = at::kFloat;
   Shape shape;
@@ -105,8 +105,7 @@ struct LayerNormBackward : public torch::autograd::Node {
     std::lock_guard<std::mutex> lock(mutex_);
     x.reset_data();
     weight.reset_data();
-    mean.reset();
-    rstd.reset();
+    stats.reset();
   }
 
   torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
@@ -139,8 +138,8 @@ struct LayerNormBackward : public torch::autograd::Node {
       ws = at::empty({bytes}, xv.options().dtype(at::kByte));
     }
     const int rc = per_layer_norm_backward(
-        &n, dy.data_ptr(), ds, xr.data_ptr(), xs, ptr_or_null(wv), mean.data_ptr<double>(),
-        rstd.data_ptr<float>(), ptr_or_null(out[0]), shape.dim, ptr_or_null(out[1]),
+        &n, dy.data_ptr(), ds, xr.data_ptr(), xs, ptr_or_null(wv), stats.data_ptr<float>(),
+        ptr_or_null(out[0]), shape.dim, ptr_or_null(out[1]),
         ptr_or_null(out[2]), ptr_or_null(ws), bytes, stream_of(xv));
     TORCH_CHECK(rc == PER_OK, error_text("per_layer_norm_backward", rc));
     return out;
@@ -214,23 +213,19 @@ Tensor layer_norm(const Tensor& x, const std::vector<int64_t>& normalized_shape,
       check_capture(b, "bias");
     }
   }
-  Tensor y, xr, mean, rstd;
+  Tensor y, xr, stats;
   {
     at::AutoDispatchBelowADInplaceOrView below;
     int64_t xs = 0;
     std::tie(xr, xs) = rows_of(x, s.norm_dims, s.dim);
     y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
-    if (grad) {
-      mean = at::empty({s.rows}, x.options().dtype(at::kDouble));
-      rstd = at::empty({s.rows}, x.options().dtype(at::kFloat));
-    }
+    if (grad) stats = at::empty({s.rows, 4}, x.options().dtype(at::kFloat));
     if (s.rows > 0 && s.dim > 0) {
       const Tensor wc = w.defined() ? w.contiguous() : w, bc = b.defined() ? b.contiguous() : b;
       const per_norm_t n{s.rows, s.dim, code_of(x.scalar_type()), code_of(param_type), (float)eps};
       check("per_layer_norm",
             per_layer_norm(&n, xr.data_ptr(), xs, ptr_or_null(wc), ptr_or_null(bc), y.data_ptr(),
-                           s.dim, grad ? mean.data_ptr<double>() : nullptr,
-                           grad ? rstd.data_ptr<float>() : nullptr, stream.stream()));
+                           s.dim, grad ? stats.data_ptr<float>() : nullptr, stream.stream()));
     }
   }
   if (grad) {
@@ -239,8 +234,7 @@ Tensor layer_norm(const Tensor& x, const std::vector<int64_t>& normalized_shape,
     node->set_next_edges(torch::autograd::collect_next_edges(x, w, b));
     node->x = torch::autograd::SavedVariable(x, false);
     if (w.defined()) node->weight = torch::autograd::SavedVariable(w, false);
-    node->mean = mean;
-    node->rstd = rstd;
+    node->stats = stats;
     node->has_weight = w.defined();
     node->has_bias = b.defined();
     node->param_type = param_type;

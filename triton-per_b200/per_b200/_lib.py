@@ -137,10 +137,10 @@ SIGNATURES = {
     "per_update_priorities_shard": (ctypes.c_int, [ctypes.POINTER(Store), i64, vp, vp, i64, vp]),
     "per_update_priorities_shard_count": (ctypes.c_int, [ctypes.POINTER(Store), i64, vp, vp, i64, vp,
                                                          vp]),
-    "per_layer_norm": (ctypes.c_int, [ctypes.POINTER(Norm), vp, i64, vp, vp, vp, i64, vp, vp, vp]),
+    "per_layer_norm": (ctypes.c_int, [ctypes.POINTER(Norm), vp, i64, vp, vp, vp, i64, vp, vp]),
     "per_layer_norm_backward_workspace": (i64, [ctypes.POINTER(Norm)]),
-    "per_layer_norm_backward": (ctypes.c_int, [ctypes.POINTER(Norm), vp, i64, vp, i64, vp, vp, vp, vp,
-                                               i64, vp, vp, vp, i64, vp]),
+    "per_layer_norm_backward": (ctypes.c_int, [ctypes.POINTER(Norm), vp, i64, vp, i64, vp, vp, vp, i64,
+                                               vp, vp, vp, i64, vp]),
     "per_grad_norm_workspace": (i64, [i64]),
     "per_grad_norm": (ctypes.c_int, [ctypes.POINTER(Tensor), i64, i32, vp, vp, i64, vp]),
     "per_scale_grads": (ctypes.c_int, [ctypes.POINTER(Tensor), i64, ctypes.c_float, vp, vp]),
