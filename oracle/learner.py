@@ -58,10 +58,14 @@ def row_error(x, rstd):
     """Rounding of a row's statistics, in units of its spread ([R, 1]).
 
     With n values, u = 2^-24 and a sum whose terms pass through at most m
-    additions, |error of the sum| <= m u sum |terms|; e = m u below. The first
-    estimate s of the mean is off by at most e avg|x|, so the shift avg(x - s)
-    is off by e (1 / rstd + e avg|x|), and the variance, relative to
-    var + eps, by e (1 + (e avg|x| rstd)^2)."""
+    additions, |error of the sum| <= m u sum |terms|; e = m u below. Distances
+    are taken from a first estimate s of the mean: of all values, off by at
+    most e avg|x|, or of a quarter of a warp's values, off by at most sqrt(3)
+    of its spread. The distances' mean square is then at most 4 / rstd^2 +
+    (e avg|x|)^2, their sums pass through at most 32 additions (half of the 64
+    in row_depth(), so that the factor 2 of their root mean square is counted),
+    and the shift avg(x - s) is off by e (1 / rstd + e avg|x|), the variance,
+    relative to var + eps, by 2 e (1 + (e avg|x| rstd)^2), which rstd halves."""
     e = row_depth(x.shape[1]) * U32
     far = e * x.double().abs().mean(1, keepdim=True) * rstd
     return e * (1 + far + far * far)

@@ -874,13 +874,6 @@ struct Outbox {
   }
 };
 
-// The forward kernel takes bulk copies where rows start anywhere or spread over
-// a cluster; whole vectors of rows in one CTA come by the threads' own cp.async
-// copies, which need no wait on a barrier and were as fast or faster
-// (32768x4096 bfloat16, float32 weights: 92 us against 115; bfloat16 weights:
-// 88 and 88; 32768x2048: 54 and 61).
-template <bool CLUSTER, bool ANY>
-constexpr bool kFwdBulk = ANY || CLUSTER;
 constexpr int kFwdStages = 3;
 // Threads that a CTA is compiled for, which bounds a thread's registers. 32
 // values of 16-bit rows with their weights and biases take some 144: CTAs of
@@ -901,17 +894,13 @@ __global__ void __launch_bounds__(THREADS) per_layer_norm_group_kernel(const Fwd
   __shared__ __align__(8) uint64_t bars[kMaxGroups][kFwdStages];
   extern __shared__ __align__(16) unsigned char dyn[];
   constexpr int VEC = 16 / sizeof(T);
-  constexpr bool kBulk = kFwdBulk<CLUSTER, ANY>;
   using R = Rows<T, NV, 1, kFwdStages, false, ANY>;
-  using C = Ring<T, VEC, NV, kFwdStages>;
   const Group<CLUSTER> t(f.group_threads, VEC, NV, f.dim);
   unsigned char* mine = dyn + t.index * (R::bytes(t.width) + (ANY ? Outbox<T, NV>::bytes(t.width) : 0));
   R rows(mine, bars[t.index], t.width);
-  C ring(dyn);
-  if constexpr (kBulk) rows.begin(t.dim, t.lane, t.width);
+  rows.begin(t.dim, t.lane, t.width);
   Turns<CLUSTER> turns;
   turns.begin(ex);
-  int stage = 0;
   const float n = (float)f.dim, inv_n = 1.f / n;
   const Array<T> x[1] = {Array<T>(f.x, f.x_stride, f.rows, f.dim, t.first)};
   T* y = static_cast<T*>(f.y) + t.first;
@@ -937,6 +926,8 @@ __global__ void __launch_bounds__(THREADS) per_layer_norm_group_kernel(const Fwd
   for (int i = 0; i < Q; ++i)
     mq[i] = all.first + 32 * i < t.warps ? values_of(all.first + 32 * i) : 0.f;
   const float inv_own = own > 0.f ? 1.f / own : 0.f;
+  const int lead = t.dim - (t.lane & ~31) * VEC;  // values of the warp's first vectors
+  const float inv_lead = lead > 0 ? 1.f / (float)(lead > 32 * VEC ? 32 * VEC : lead) : 0.f;
 
   if constexpr (CLUSTER)
     cluster_sync();  // before a CTA writes into another one's shared memory, that one has to run
@@ -944,16 +935,7 @@ __global__ void __launch_bounds__(THREADS) per_layer_norm_group_kernel(const Fwd
     __syncthreads();
   per_wait_previous_grid();
   auto fetch = [&](int st, int64_t row) {
-    if constexpr (kBulk) {
-      rows.fetch(st, x, nullptr, row, t.dim, t.lane, t.width, row < f.rows);
-    } else {
-#pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        const int c = (t.lane + k * t.width) * VEC;
-        ring.fetch(st, k, x[0].row(row) + c, row < f.rows && c < t.dim);
-      }
-      C::commit();
-    }
+    rows.fetch(st, x, nullptr, row, t.dim, t.lane, t.width, row < f.rows);
   };
   for (int k = 0; k < kFwdStages; ++k) fetch(k, t.base + k * t.step);
   if constexpr (ANY) cta_part_sync(t);  // values that were fetched one by one
@@ -967,38 +949,28 @@ __global__ void __launch_bounds__(THREADS) per_layer_norm_group_kernel(const Fwd
       keep_packed(w);
       keep_packed(b);
     }
-    if constexpr (kBulk)
-      rows.wait(x, row);
-    else
-      C::wait();
+    rows.wait(x, row);
     {
       Pack<T, VEC> q[NV];
 #pragma unroll
-      for (int k = 0; k < NV; ++k)
-        if constexpr (kBulk)
-          q[k] = rows.get(0, k, t.dim, t.lane, t.width);
-        else
-          q[k] = ring.get(stage, k);
+      for (int k = 0; k < NV; ++k) q[k] = rows.get(0, k, t.dim, t.lane, t.width);
 #pragma unroll
-      for (int i = 0; i < NV * VEC / 2; ++i) {
-        v[i] = get2(q, i);
-        a = per_add2(a, v[i]);
-      }
+      for (int i = 0; i < NV * VEC / 2; ++i) v[i] = get2(q, i);
+#pragma unroll
+      for (int i = 0; i < VEC / 2; ++i) a = per_add2(a, v[i]);
     }
-    if constexpr (!kBulk) {
-      fetch(stage, row + kFwdStages * t.step);
-      stage = stage + 1 == kFwdStages ? 0 : stage + 1;
-    }
-    // Distances from the warp's own mean first. Warp q of m_q values then has the mean
-    // s_q + u_q with u_q = d1_q / m_q, and squares around it d2_q - d1_q u_q. Seen from s_0 its
-    // mean lies at z_q; the row's at z = sum m_q z_q / n, and the row's squares are the warps'
-    // plus m_q (z_q - z)^2 each.
-    const float s = over(lanes_sum<32>(a.x + a.y), own, inv_own);
+    // Distances from a mean of the warp's own first: of its first vectors alone, a part 1 / NV of
+    // its values or more, whose mean lies within sqrt(NV - 1) standard deviations of the warp's,
+    // so that the subtraction in its squares below loses no more than 2 bits (NV 4). Warp q of m_q
+    // values then has the mean s_q + u_q with u_q = d1_q / m_q, and squares around it
+    // d2_q - d1_q u_q. Seen from s_0 its mean lies at z_q; the row's at z = sum m_q z_q / n, and the
+    // row's squares are the warps' plus m_q (z_q - z)^2 each.
+    const float s = lanes_sum<32>(a.x + a.y) * inv_lead;
     const float2 e = centre<VEC, NV>(v, s, t.lane, t.width, t.dim);
     const float e1 = lanes_sum<32>(e.x), e2 = lanes_sum<32>(e.y);
-    const float u = e1 * inv_own;
+    const float u = over(e1, own, inv_own);
     put(ex, turns, t, make_float4(s, u, fmaxf(fmaf(-e1, u, e2), 0.f), 0.f));
-    if constexpr (kBulk) fetch(rows.stage, row + kFwdStages * t.step);
+    fetch(rows.stage, row + kFwdStages * t.step);
     const float s0 = ex.slot[turns.turn][all.from].x;
     float z = 0.f, sq = 0.f, zq[Q];
 #pragma unroll
@@ -1017,7 +989,7 @@ __global__ void __launch_bounds__(THREADS) per_layer_norm_group_kernel(const Fwd
     for (int i = 0; i < Q; ++i) sq = fmaf(mq[i] * (zq[i] - z), zq[i] - z, sq);
     const float var = all.sum(sq) * inv_n;
     float r = rsqrtf(fmaxf(var, 0.f) + f.eps);
-    if ((kBulk && rows.failed) || turns.failed) r = __int_as_float(0x7fc00000);  // something never came: say so in the result
+    if (rows.failed || turns.failed) r = __int_as_float(0x7fc00000);  // something never came: say so in the result
     Pack<T, VEC> o[NV];
     normed<T, P, VEC, NV>(o, v, z - (s - s0), r, w, b);
     if constexpr (ANY)
@@ -1025,9 +997,9 @@ __global__ void __launch_bounds__(THREADS) per_layer_norm_group_kernel(const Fwd
     else
       store_row(y + row * f.y_stride, o, t.lane, t.width, t.dim);
     if (f.stats && t.lane == 0 && t.first == 0) f.stats[row] = make_float4(s0, z, r, 0.f);
-    if constexpr (kBulk) rows.next();
+    rows.next();
   }
-  if constexpr (kBulk) rows.end();
+  rows.end();
   if constexpr (CLUSTER) cluster_sync();  // no CTA ends while another may still write to it
 }
 
@@ -1370,11 +1342,9 @@ int forward_group(const Shape& s, const Fwd& in, cudaStream_t stream) {
     if (s.threads <= 192)
       fn = (const void*)per_layer_norm_group_kernel<T, P, NV, CLUSTER, ANY, kWideThreads>;
   // rows of few threads share a CTA of about 128
-  const int groups = CLUSTER || !ANY || s.threads > 64 ? 1 : 128 / s.threads;
-  const size_t smem = kFwdBulk<CLUSTER, ANY>
-                          ? groups * (Rows<T, NV, 1, kFwdStages, false, ANY>::bytes(s.threads) +
-                                      (ANY ? Outbox<T, NV>::bytes(s.threads) : 0))
-                          : Ring<T, 16 / sizeof(T), NV, kFwdStages>::kBytes * s.threads;
+  const int groups = CLUSTER || s.threads > 64 ? 1 : 128 / s.threads;
+  const size_t smem = groups * (Rows<T, NV, 1, kFwdStages, false, ANY>::bytes(s.threads) +
+                                (ANY ? Outbox<T, NV>::bytes(s.threads) : 0));
   int64_t grid = 0;
   const int rc = row_ctas(fn, s, s.threads * groups, smem, f.rows, 0, &grid);
   return rc ? rc : launch(fn, grid * s.ctas, s.threads * groups, smem, &f, stream, s.ctas);
