@@ -329,7 +329,7 @@ int per_update_priorities_shard_count(const per_store_t* store, int64_t base, co
  * the types; a 16-bit result is rounded once. */
 typedef struct per_norm {
   int64_t rows;         /* >= 0 */
-  int64_t dim;          /* 1 .. 2^31 - 1 */
+  int64_t dim;          /* 1 .. 2^30 */
   int32_t dtype;        /* PER_* type of x, y, dy, dx */
   int32_t param_dtype;  /* PER_* type of weight, bias and their gradients: PER_F32 or `dtype` */
   float eps;            /* >= 0, added to the variance (forward only) */

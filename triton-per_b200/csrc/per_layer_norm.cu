@@ -42,10 +42,13 @@ struct Bwd {
   void* dx;
   void* dw;
   void* db;
-  float* part;  // [splits][2][dim]
+  float* part;  // [splits][2][padded]: sums of dw and db, in the order of `places`
   int64_t rows, dy_stride, x_stride, dx_stride;
   int32_t dim, splits;
   int32_t group_threads;  // of a row that spans warps
+  struct Places {         // the order of the columns in a partial row, see store_columns()
+    int32_t padded, slice, width, vec;
+  } places;
 };
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -262,17 +265,45 @@ __device__ __forceinline__ void backward_values(Pack<T, VEC> (&o)[NV], const flo
   for (int i = 0; i < NV * VEC / 2; ++i) set2(o, i, per_fma2(h[i], k1, per_fma2(g[i], r2, k0)));
 }
 
-// f(column of a value, dw, db) for a thread's column sums
-template <int VEC, int NV, typename F>
-__device__ __forceinline__ void for_columns(const float2 (&aw)[NV * VEC / 2],
-                                            const float2 (&ab)[NV * VEC / 2], int lane, int width,
-                                            int dim, F f) {
+// A thread's column sums into a partial row: four neighbouring columns at a
+// time, thread after thread, so that a warp's stores are whole lines (column by
+// column a thread's stores lie 16 or 32 bytes from its neighbour's: the partial
+// rows of 16384x8192 bfloat16 took 17 us to write and join, 7 us so). Columns
+// beyond the row are stored too, and not looked at.
+template <int VEC, int NV>
+__device__ __forceinline__ void store_columns(float* part, const float2 (&a)[NV * VEC / 2], int lane,
+                                              int width) {
+  if constexpr (VEC > 1) {
 #pragma unroll
-  for (int i = 0; i < NV * VEC / 2; ++i) {
-    const int c0 = (lane + 2 * i / VEC * width) * VEC + 2 * i % VEC;
-    const int c1 = VEC > 1 ? c0 + 1 : lane + (2 * i + 1) * width;
-    if (c0 < dim) f(c0, aw[i].x, ab[i].x);
-    if (c1 < dim) f(c1, aw[i].y, ab[i].y);
+    for (int q = 0; q < NV * VEC / 4; ++q)
+      reinterpret_cast<float4*>(part)[q * width + lane] =
+          make_float4(a[2 * q].x, a[2 * q].y, a[2 * q + 1].x, a[2 * q + 1].y);
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV / 2; ++i) {
+      part[2 * i * width + lane] = a[i].x;
+      part[(2 * i + 1) * width + lane] = a[i].y;
+    }
+  }
+}
+// The column that place p of a partial row holds.
+__device__ __forceinline__ int column_at(const Bwd::Places& o, int p) {
+  const int cta = p / o.slice, r = p % o.slice;
+  if (o.vec == 1) return p;
+  const int q = r / 4 / o.width, lane = r / 4 % o.width, per = o.vec / 4;
+  return cta * o.slice + (lane + q / per * o.width) * o.vec + q % per * 4 + r % 4;
+}
+
+// The partial rows [groups][2][padded] of a CTA's groups, in shared memory,
+// added into one.
+__device__ __forceinline__ void add_groups(float* part, const float* sums, int groups, int padded) {
+  for (int c = threadIdx.x; c < padded / 2; c += blockDim.x) {
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int q = 0; q < groups; ++q) {
+      const float4 u = reinterpret_cast<const float4*>(sums)[q * (padded / 2) + c];
+      v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+    }
+    reinterpret_cast<float4*>(part)[c] = v;
   }
 }
 
@@ -455,9 +486,9 @@ __global__ void __launch_bounds__(256) per_layer_norm_backward_warp_kernel(const
   if (!g.part) return;
   // the row groups of a warp by shuffles, then the warps through shared
   // memory, where the (empty) copies still in flight have ended
-  float* part = g.part + (int64_t)blockIdx.x * 2 * g.dim;
-  float* sums = reinterpret_cast<float*>(dyn);  // [warps][2][dim]
-  float* own = sums + (threadIdx.x >> 5) * 2 * g.dim;
+  constexpr int kPadded = LANES * NV * VEC;
+  float* sums = reinterpret_cast<float*>(dyn);  // [warps][2][padded]
+  float* own = sums + (threadIdx.x >> 5) * 2 * kPadded;
   asm volatile("cp.async.wait_all;" ::: "memory");
   __syncthreads();
 #pragma unroll
@@ -469,17 +500,12 @@ __global__ void __launch_bounds__(256) per_layer_norm_backward_warp_kernel(const
       ab[i].x += __shfl_xor_sync(PER_FULL_MASK, ab[i].x, o);
       ab[i].y += __shfl_xor_sync(PER_FULL_MASK, ab[i].y, o);
     }
-  if (mine == 0)
-    for_columns<VEC, NV>(aw, ab, lane, LANES, g.dim, [&](int c, float dw, float db) {
-      own[c] = dw;
-      own[g.dim + c] = db;
-    });
-  __syncthreads();
-  for (int c = threadIdx.x; c < 2 * g.dim; c += blockDim.x) {
-    float v = 0.f;
-    for (int q = 0; q < (int)(blockDim.x >> 5); ++q) v += sums[q * 2 * g.dim + c];
-    part[c] = v;
+  if (mine == 0) {
+    store_columns<VEC, NV>(own, aw, lane, LANES);
+    store_columns<VEC, NV>(own + kPadded, ab, lane, LANES);
   }
+  __syncthreads();
+  add_groups(g.part + (int64_t)blockIdx.x * 2 * kPadded, sums, blockDim.x >> 5, kPadded);
 }
 
 // ---- longer rows: a group of warps per row (several groups in a CTA), or a
@@ -1073,28 +1099,18 @@ __global__ void __launch_bounds__(kRowThreads) per_layer_norm_backward_group_ker
   rows.end();
   if constexpr (CLUSTER) cluster_sync();  // no CTA ends while another may still write to it
   if (!g.part) return;
+  const int slice = t.width * NV * VEC;  // places of this CTA's part of the row
   if (CLUSTER || t.width == (int)blockDim.x) {
-    float* part = g.part + t.base * 2 * g.dim + t.first;
-    for_columns<VEC, NV>(aw, ab, t.lane, t.width, t.dim, [&](int c, float dw, float db) {
-      part[c] = dw;
-      part[g.dim + c] = db;
-    });
+    float* part = g.part + t.base * 2 * g.places.padded + t.first;
+    store_columns<VEC, NV>(part, aw, t.lane, t.width);
+    store_columns<VEC, NV>(part + g.places.padded, ab, t.lane, t.width);
   } else {
-    float* part = g.part + (int64_t)blockIdx.x * 2 * g.dim;
-    float* sums = reinterpret_cast<float*>(dyn);  // [groups][2][dim], over the slots, all of them read
-    float* mine = sums + t.index * 2 * g.dim;
+    float* sums = reinterpret_cast<float*>(dyn);  // [groups][2][padded], over the slots, all of them read
     __syncthreads();
-    for_columns<VEC, NV>(aw, ab, t.lane, t.width, t.dim, [&](int c, float dw, float db) {
-      mine[c] = dw;
-      mine[g.dim + c] = db;
-    });
+    store_columns<VEC, NV>(sums + t.index * 2 * slice, aw, t.lane, t.width);
+    store_columns<VEC, NV>(sums + t.index * 2 * slice + slice, ab, t.lane, t.width);
     __syncthreads();
-    const int groups = blockDim.x / t.width;
-    for (int c = threadIdx.x; c < 2 * g.dim; c += blockDim.x) {
-      float v = 0.f;
-      for (int q = 0; q < groups; ++q) v += sums[q * 2 * g.dim + c];
-      part[c] = v;
-    }
+    add_groups(g.part + (int64_t)blockIdx.x * 2 * slice, sums, blockDim.x / t.width, slice);
   }
 }
 
@@ -1177,32 +1193,47 @@ __global__ void __launch_bounds__(kThreads) per_layer_norm_dw_long_kernel(const 
     dw = fmaf(v, (per_to_f32(x[row * g.x_stride]) - hi - lo) * r, dw);
     db += v;
   }
-  g.part[(int64_t)split * 2 * g.dim + c] = dw;
-  g.part[((int64_t)split * 2 + 1) * g.dim + c] = db;
+  g.part[(int64_t)split * 2 * g.places.padded + c] = dw;
+  g.part[((int64_t)split * 2 + 1) * g.places.padded + c] = db;
 }
 
-// dw and db from the partial rows: a CTA adds 32 columns, each of its 8 warps
-// every eighth partial row, then the warps' sums in order.
-constexpr int kJoinThreads = 256;
+// dw and db from the partial rows. A CTA adds 32 places: 8 threads take four
+// each of a partial row, its 64 such teams every 64th row, so that most lists
+// are read in a few loads per thread; the teams' sums are added in order.
+constexpr int kJoinThreads = 512;
 template <typename P>
 __global__ void __launch_bounds__(kJoinThreads) per_layer_norm_join_kernel(const Bwd g) {
   __shared__ float s[kJoinThreads / 32][32];
   per_wait_previous_grid();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t c = (int64_t)blockIdx.x * 32 + lane;  // column of [dw, db]
-  const int64_t cols = 2 * (int64_t)g.dim;
-  float v = 0.f;
-  if (c < cols) {
-#pragma unroll 8
-    for (int k = warp; k < g.splits; k += kJoinThreads / 32) v += g.part[k * cols + c];
+  const int quad = threadIdx.x & 7, team = threadIdx.x >> 3;
+  const int64_t all = 2 * (int64_t)g.places.padded;
+  const int64_t at = (int64_t)blockIdx.x * 32 + quad * 4;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (at < all) {
+#pragma unroll 4
+    for (int k = team; k < g.splits; k += kJoinThreads / 8) {
+      const float4 u = *reinterpret_cast<const float4*>(g.part + k * all + at);
+      v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+    }
   }
-  s[warp][lane] = v;
-  __syncthreads();
-  if (warp || c >= cols) return;
 #pragma unroll
-  for (int q = 1; q < kJoinThreads / 32; ++q) v += s[q][lane];
-  void* out = c < g.dim ? g.dw : g.db;
-  if (out) static_cast<P*>(out)[c < g.dim ? c : c - g.dim] = per_from_f32<P>(v);
+  for (int o = 8; o < 32; o <<= 1) {
+    v.x += __shfl_xor_sync(PER_FULL_MASK, v.x, o);
+    v.y += __shfl_xor_sync(PER_FULL_MASK, v.y, o);
+    v.z += __shfl_xor_sync(PER_FULL_MASK, v.z, o);
+    v.w += __shfl_xor_sync(PER_FULL_MASK, v.w, o);
+  }
+  if ((threadIdx.x & 31) < 8) *reinterpret_cast<float4*>(&s[threadIdx.x >> 5][quad * 4]) = v;
+  __syncthreads();
+  const int64_t p = (int64_t)blockIdx.x * 32 + threadIdx.x;
+  if (threadIdx.x >= 32 || p >= all) return;
+  float sum = s[0][threadIdx.x];
+#pragma unroll
+  for (int q = 1; q < kJoinThreads / 32; ++q) sum += s[q][threadIdx.x];
+  const bool second = p >= g.places.padded;
+  const int c = column_at(g.places, (int)(second ? p - g.places.padded : p));
+  void* out = second ? g.db : g.dw;
+  if (out && c < g.dim) static_cast<P*>(out)[c] = per_from_f32<P>(sum);
 }
 
 int launch(const void* fn, int64_t grid, int threads, size_t smem, const void* arg,
@@ -1375,6 +1406,17 @@ int64_t most_partials(int64_t rows, int64_t dim) {
   return rows < most ? rows : most;
 }
 
+Bwd::Places long_places(int32_t dim) {
+  const int32_t padded = (dim - 1) / 4 * 4 + 4;
+  return {padded, padded, 1, 1};
+}
+
+// The order of the columns in a partial row.
+Bwd::Places places_of(const Shape& s, int vec) {
+  const int slice = (s.lanes ? s.lanes : s.threads) * s.nv * vec;
+  return {s.ctas * slice, slice, s.lanes ? s.lanes : s.threads, vec};
+}
+
 // The row kernel, then the join of its partial rows where columns are wanted.
 template <typename P>
 int backward_run(const void* fn, const Shape& s, int threads, size_t smem, Bwd g, cudaStream_t stream) {
@@ -1386,14 +1428,16 @@ int backward_run(const void* fn, const Shape& s, int threads, size_t smem, Bwd g
   rc = launch(fn, grid * s.ctas, threads, smem, &g, stream, s.ctas);
   if (rc || !columns) return rc;
   g.splits = (int32_t)grid;
-  return launch((const void*)per_layer_norm_join_kernel<P>, (2 * (int64_t)g.dim - 1) / 32 + 1,
+  return launch((const void*)per_layer_norm_join_kernel<P>, (2 * (int64_t)g.places.padded - 1) / 32 + 1,
                 kJoinThreads, 0, &g, stream);
 }
 
 template <typename T, typename P, int VEC, int NV, int LANES>
-int backward_warp(const Shape& s, const Bwd& g, cudaStream_t stream) {
+int backward_warp(const Shape& s, const Bwd& in, cudaStream_t stream) {
+  Bwd g = in;
+  g.places = places_of(s, VEC);
   const size_t ring = Ring<T, VEC, 2 * NV, kWarpStages>::kBytes * s.threads;
-  const size_t sums = (size_t)(s.threads / 32) * 2 * g.dim * 4;
+  const size_t sums = (size_t)(s.threads / 32) * 2 * g.places.padded * 4;
   return backward_run<P>((const void*)per_layer_norm_backward_warp_kernel<T, P, VEC, NV, LANES>, s,
                          s.threads, ring > sums ? ring : sums, g, stream);
 }
@@ -1407,7 +1451,8 @@ int backward_group(const Shape& s, const Bwd& in, cudaStream_t stream) {
   groups = groups > kMaxGroups ? kMaxGroups : groups;
   size_t smem = groups * (Rows<T, NV, 2, kBwdStages<ANY>, true, ANY>::bytes(s.threads) +
                           (ANY ? Outbox<T, NV>::bytes(s.threads) : 0));
-  const size_t sums = groups > 1 ? (size_t)groups * 2 * g.dim * 4 : 0;
+  g.places = places_of(s, 16 / sizeof(T));
+  const size_t sums = groups > 1 ? (size_t)groups * 2 * g.places.padded * 4 : 0;
   smem = smem > sums ? smem : sums;
   return backward_run<P>((const void*)per_layer_norm_backward_group_kernel<T, P, NV, CLUSTER, ANY>, s,
                          s.threads * groups, smem, g, stream);
@@ -1421,6 +1466,7 @@ int backward_rows(const Bwd& in, cudaStream_t stream) {
   if (PER_NORM_SHAPE(s, rc, backward_warp, backward_group, T, P, ANY, FULL, in, stream)) return rc;
   Bwd g = in;
   g.splits = splits_of(g.rows, g.dim);
+  g.places = long_places(g.dim);
   if (g.dx)
     rc = launch((const void*)per_layer_norm_dx_long_kernel<T, P>, row_grid(g.rows), kThreads, 0,
                 &g, stream);
@@ -1429,7 +1475,7 @@ int backward_rows(const Bwd& in, cudaStream_t stream) {
   rc = launch((const void*)per_layer_norm_dw_long_kernel<T>, tiles * g.splits, kThreads, 0, &g,
               stream);
   if (rc) return rc;
-  return launch((const void*)per_layer_norm_join_kernel<P>, (2 * (int64_t)g.dim - 1) / 32 + 1,
+  return launch((const void*)per_layer_norm_join_kernel<P>, (2 * (int64_t)g.places.padded - 1) / 32 + 1,
                 kJoinThreads, 0, &g, stream);
 }
 
@@ -1440,6 +1486,23 @@ int backward(const Bwd& g, cudaStream_t stream) {
       aligned(g.w, 0, 1))
     return backward_rows<T, P, false>(g, stream);
   return backward_rows<T, P, true>(g, stream);
+}
+
+// Bytes of partial rows, whichever kernel the pointers' alignment asks for.
+template <typename T, typename P>
+int64_t backward_bytes(const per_norm_t& n) {
+  if (n.rows == 0) return 0;
+  constexpr int VEC = 16 / sizeof(T), FULL = kBwdVectors<T>;
+  int64_t most = 0;
+  for (const bool any : {false, true}) {
+    if (!any && n.dim % VEC) continue;
+    const Shape s = shape_of(n.dim, VEC, any, any, FULL, kRowThreads, 256);
+    const int64_t bytes =
+        s.ctas ? most_partials(n.rows, n.dim) * places_of(s, any && s.lanes ? 1 : VEC).padded
+               : (int64_t)splits_of(n.rows, n.dim) * long_places((int32_t)n.dim).padded;
+    most = bytes > most ? bytes : most;
+  }
+  return most * 2 * 4;
 }
 
 }  // namespace
@@ -1461,10 +1524,7 @@ int per_launch_layer_norm(const per_norm_t& n, const void* x, int64_t x_stride, 
 }
 
 int64_t per_layer_norm_backward_bytes(const per_norm_t& n) {
-  int64_t most = most_partials(n.rows, n.dim);
-  const int64_t s = splits_of(n.rows, n.dim);
-  if (most < s) most = s;
-  return most * 2 * n.dim * 4;
+  return PER_NORM_TYPES(n, backward_bytes, n);
 }
 
 int per_launch_layer_norm_backward(const per_norm_t& n, const void* dy, int64_t dy_stride,
@@ -1474,6 +1534,6 @@ int per_launch_layer_norm_backward(const per_norm_t& n, const void* dy, int64_t 
                                    cudaStream_t stream) {
   const Bwd g{dy, x, weight, reinterpret_cast<const float4*>(stats), dx, dweight, dbias,
               static_cast<float*>(workspace),
-              n.rows, dy_stride, x_stride, dx_stride, (int32_t)n.dim, 0, 0};
+              n.rows, dy_stride, x_stride, dx_stride, (int32_t)n.dim, 0, 0, {}};
   return PER_NORM_TYPES(n, backward, g, stream);
 }

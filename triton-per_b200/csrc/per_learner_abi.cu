@@ -8,7 +8,7 @@
 
 namespace {
 
-constexpr int64_t kMaxDim = 0x7fffffffLL;
+constexpr int64_t kMaxDim = (int64_t)1 << 30;
 
 int check_norm(const per_norm_t* n) {
   if (!n) return PER_ERR_NULL_POINTER;

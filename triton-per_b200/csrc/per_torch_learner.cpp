@@ -4,6 +4,7 @@
 // (one workspace per call, so calls on different streams and captured graphs
 // share none) and calls the C ABI. No kernels here.
 #include <torch/extension.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/function.h>
@@ -45,6 +46,12 @@ int32_t code_of(at::ScalarType t) {
 
 void* stream_of(const Tensor& t) {
   return c10::cuda::getCurrentCUDAStream(t.get_device()).stream();
+}
+
+// A new tensor on the current stream, without the dispatcher's detour (about
+// 1 us of host time less than at::empty, of which a training step makes six).
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, c10::Device device) {
+  return Tensor(at::detail::empty_cuda(sizes, type, device, std::nullopt));
 }
 
 // ------------------------------------------------------------- layer norm
@@ -125,17 +132,17 @@ struct LayerNormBackward : public torch::autograd::Node {
                 "per_b200.layer_norm: the gradient must have the input's type and device");
     const auto [xr, xs] = rows_of(xv, shape.norm_dims, shape.dim);
     const auto [dy, ds] = rows_of(grads[0], shape.norm_dims, shape.dim, true);
-    if (want_x) out[0] = at::empty(xv.sizes(), xv.options().memory_format(at::MemoryFormat::Contiguous));
+    if (want_x) out[0] = fresh(xv.sizes(), xv.scalar_type(), xv.device());
     const auto norm_sizes = xv.sizes().slice(xv.dim() - shape.norm_dims);
-    if (want_w) out[1] = at::empty(norm_sizes, xv.options().dtype(param_type));
-    if (want_b) out[2] = at::empty(norm_sizes, xv.options().dtype(param_type));
+    if (want_w) out[1] = fresh(norm_sizes, param_type, xv.device());
+    if (want_b) out[2] = fresh(norm_sizes, param_type, xv.device());
     if (shape.dim == 0) return out;
     const per_norm_t n{shape.rows, shape.dim, code_of(xv.scalar_type()), code_of(param_type), 0.f};
     int64_t bytes = 0;
     Tensor ws;
     if (shape.rows > 0) {
       bytes = per_layer_norm_backward_workspace(&n);
-      ws = at::empty({bytes}, xv.options().dtype(at::kByte));
+      ws = fresh({bytes}, at::kByte, xv.device());
     }
     const int rc = per_layer_norm_backward(
         &n, dy.data_ptr(), ds, xr.data_ptr(), xs, ptr_or_null(wv), stats.data_ptr<float>(),
@@ -218,8 +225,8 @@ Tensor layer_norm(const Tensor& x, const std::vector<int64_t>& normalized_shape,
     at::AutoDispatchBelowADInplaceOrView below;
     int64_t xs = 0;
     std::tie(xr, xs) = rows_of(x, s.norm_dims, s.dim);
-    y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
-    if (grad) stats = at::empty({s.rows, 4}, x.options().dtype(at::kFloat));
+    y = fresh(x.sizes(), x.scalar_type(), x.device());
+    if (grad) stats = fresh({s.rows, 4}, at::kFloat, x.device());
     if (s.rows > 0 && s.dim > 0) {
       const Tensor wc = w.defined() ? w.contiguous() : w, bc = b.defined() ? b.contiguous() : b;
       const per_norm_t n{s.rows, s.dim, code_of(x.scalar_type()), code_of(param_type), (float)eps};
@@ -295,7 +302,6 @@ struct List {
   }
 
   void* stream() const { return c10::cuda::getCurrentCUDAStream(device.index()).stream(); }
-  at::TensorOptions options() const { return at::TensorOptions().device(device); }
   // the tensors have been written to
   void written() const {
     for (at::TensorImpl* g : impl)
@@ -321,8 +327,7 @@ List list_of(const py::list& tensors, bool take_grads, const char* what) {
 
 std::pair<Tensor, Tensor> norm_and_workspace(const List& l, int64_t* bytes) {
   *bytes = per_grad_norm_workspace((int64_t)l.t.size());
-  return {at::empty({}, l.options().dtype(at::kFloat)),
-          at::empty({*bytes}, l.options().dtype(at::kByte))};
+  return {fresh({}, at::kFloat, l.device), fresh({*bytes}, at::kByte, l.device)};
 }
 
 // grad_norm(tensors, kind) -> float32 scalar on the device; None for an empty list
