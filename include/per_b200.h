@@ -394,7 +394,7 @@ int per_grad_norm(const per_tensor_t* tensors, int64_t n, int32_t kind, float* n
  * rounded once; tensors are not touched where that factor is 1. `norm` is a
  * device float32 (of per_grad_norm(), or joined over the ranks of a job). The
  * factor is NaN where *norm is NaN, and 0 where it is infinite. No two tensors
- * may overlap. */
+ * may overlap, nor may *norm be part of one. */
 int per_scale_grads(const per_tensor_t* tensors, int64_t n, float max_norm, const float* norm,
                     void* stream);
 

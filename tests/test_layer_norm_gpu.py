@@ -273,6 +273,163 @@ def test_same_bits_every_time():
             assert torch.equal(a, c)
 
 
+def test_weights_with_gaps_and_in_another_order():
+    for dim in (24, 300, 2048):
+        x, dy = normal(17, dim), normal(17, dim, seed=1)
+        spread = normal(dim, 3, seed=2)
+        w, b = spread[:, 1], spread[:, 2]
+        check_forward(x, w, b)
+        check_train(x, w, b, dy)
+    x, dy = normal(9, 5, 6), normal(9, 5, 6, seed=1)
+    w = normal(6, 5, seed=2).t()  # [5, 6], columns first
+    leaves = [x.clone().requires_grad_(), w.detach().requires_grad_()]
+    y = per_b200.layer_norm(leaves[0], (5, 6), leaves[1])
+    y.backward(dy)
+    flat = lambda t: t.detach().reshape(-1, 30)  # noqa: E731
+    want, bound = ref.layer_norm_bound(flat(x), flat(w)[0], None, EPS, F32)
+    close(flat(y), want, bound, "y")
+    dx, dw, _ = ref.layer_norm_backward_bound(flat(dy), flat(x), flat(w)[0], EPS, F32, F32)
+    close(flat(leaves[0].grad), *dx, "dx")
+    close(flat(leaves[1].grad)[0], *dw, "dw")
+
+
+@pytest.mark.parametrize("dim", [40, 1001, 1024, 5001, 20001, 70001])
+def test_one_gradient_row_for_all(dim):
+    """An upstream gradient of stride 0 over the rows, read where it lies."""
+    for dtype in (F32, BF16):
+        x = rows_like_activations(7, dim, dtype)
+        w, b = params_like(dim, F32, "both")
+        check_train(x, w, b, normal(1, dim, seed=8).to(dtype).expand(7, dim))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("dim", [40, 77, 1000, 1001, 9000, 9001, 20000, 20001, 70001])
+def test_each_gradient_alone(dtype, dim):
+    x, dy = rows_like_activations(23, dim, dtype), normal(23, dim, seed=1).to(dtype)
+    w, b = params_like(dim, F32, "both")
+    full = check_train(x, w, b, dy)
+    for k in range(3):
+        leaves = [t.clone().requires_grad_(i == k) for i, t in enumerate((x, w, b))]
+        per_b200.layer_norm(leaves[0], dim, leaves[1], leaves[2]).backward(dy)
+        assert torch.equal(leaves[k].grad, full[k])
+
+
+@pytest.mark.parametrize("dim", [3, 20, 70, 600, 3000])
+def test_output_beside_the_input_in_one_buffer(dim):
+    """The C entry point writes columns between the ones it reads, and nothing else."""
+    from per_b200 import _lib
+
+    for dtype, code in ((F32, 0), (BF16, 1)):
+        for gap in (0, 1, 5):
+            width = 2 * dim + 3 * gap + 1
+            buf = normal(50, width).to(dtype)
+            old = buf.clone()
+            eb = buf.element_size()
+            n = _lib.Norm(50, dim, code, code, EPS)
+            rc = _lib.lib.per_layer_norm(n, buf.data_ptr() + gap * eb, width, None, None,
+                                         buf.data_ptr() + (2 * gap + dim) * eb, width, None,
+                                         torch.cuda.current_stream().cuda_stream)
+            assert rc == 0
+            torch.cuda.synchronize()
+            want, bound = ref.layer_norm_bound(old[:, gap:gap + dim], None, None, EPS, dtype)
+            got = buf[:, 2 * gap + dim:2 * gap + 2 * dim]
+            close(got, want, bound, "y")
+            buf[:, 2 * gap + dim:2 * gap + 2 * dim] = old[:, 2 * gap + dim:2 * gap + 2 * dim]
+            assert torch.equal(buf, old)
+
+
+def test_rows_beyond_the_workspace_of_a_wave():
+    """Millions of short rows: each thread's row walks far."""
+    x = normal(3_000_000, 8)
+    w, b = params_like(8, F32, "both")
+    check_train(x, w, b, normal(3_000_000, 8, seed=1))
+
+
+def test_recomputed_activations():
+    from torch.utils.checkpoint import checkpoint
+
+    m = torch.nn.Sequential(torch.nn.Linear(64, 64), per_b200.LayerNorm(64), torch.nn.ReLU()).cuda()
+    x = normal(30, 64).requires_grad_()
+    want = torch.autograd.grad(m(x).square().sum(), [x, *m.parameters()])
+    got = torch.autograd.grad(checkpoint(m, x, use_reentrant=False).square().sum(), [x, *m.parameters()])
+    for a, b in zip(want, got):
+        assert torch.equal(a, b)
+
+
+def test_calls_from_several_threads():
+    import threading
+
+    x, w = normal(2000, 777), torch.ones(777, device="cuda")
+    want = per_b200.layer_norm(x, 777, w)
+    leaf = x.clone().requires_grad_()
+    wantg, = torch.autograd.grad(per_b200.layer_norm(leaf, 777, w).square().sum(), [leaf])
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(k):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                leaf = x.clone().requires_grad_()
+                y = per_b200.layer_norm(leaf, 777, w)
+                g, = torch.autograd.grad(y.square().sum(), [leaf])
+                n = per_b200.grad_norm([g])
+                s.synchronize()
+                if not torch.equal(y, want) or not torch.equal(g, wantg) or not float(n) > 0:
+                    wrong.append(k)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not wrong
+
+
+FIRST_CALL = """
+import sys
+sys.path.insert(0, {path!r})
+import torch, per_b200
+x = torch.randn(300, {dim}, device="cuda", requires_grad=True)
+w = torch.ones({dim}, device="cuda", requires_grad=True)
+b = torch.zeros({dim}, device="cuda", requires_grad=True)
+p = [torch.nn.Parameter(torch.randn(n, device="cuda")) for n in {sizes}]
+for q in p:
+    q.grad = torch.randn_like(q)
+start = [q.grad.clone() for q in p]
+dy = torch.randn(300, {dim}, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    y = per_b200.layer_norm(x, {dim}, w, b)
+    grads = torch.autograd.grad(y, (x, w, b), dy)
+    norm = per_b200.clip_grad_norm_(p, 0.5)
+g.replay()
+torch.cuda.synchronize()
+y2 = per_b200.layer_norm(x, {dim}, w, b)
+for a, c in zip(grads, torch.autograd.grad(y2, (x, w, b), dy)):
+    assert torch.equal(a, c)
+assert torch.equal(y, y2)
+clipped = [q.grad.clone() for q in p]
+for q, s in zip(p, start):
+    q.grad.copy_(s)
+assert torch.equal(per_b200.clip_grad_norm_(p, 0.5), norm)
+for q, c in zip(p, clipped):
+    assert torch.equal(q.grad, c)
+print("fine")
+"""
+
+
+@pytest.mark.parametrize("dim,sizes", [(256, [1000, 7]), (1001, [3_000_000, 5]), (20000, [100] * 300)])
+def test_first_call_of_a_process_is_captured(dim, sizes):
+    import os
+    import subprocess
+    import sys
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "triton-per_b200")
+    out = subprocess.run([sys.executable, "-c", FIRST_CALL.format(path=path, dim=dim, sizes=sizes)],
+                         capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "fine" in out.stdout, out.stderr[-2000:]
+
+
 def test_second_derivative_is_refused():
     x = normal(4, 8).requires_grad_()
     y = per_b200.layer_norm(x, 8)

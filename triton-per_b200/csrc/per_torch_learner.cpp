@@ -123,7 +123,7 @@ struct LayerNormBackward : public torch::autograd::Node {
                 "per_b200.layer_norm: its gradient is not differentiable again "
                 "(backward with create_graph=True)");
     const Tensor xv = x.unpack();
-    const Tensor wv = has_weight ? weight.unpack() : Tensor();
+    const Tensor wv = has_weight ? weight.unpack().contiguous() : Tensor();
     const bool want_x = task_should_compute_output(0);
     const bool want_w = has_weight && task_should_compute_output(1);
     const bool want_b = has_bias && task_should_compute_output(2);

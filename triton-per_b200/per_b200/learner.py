@@ -94,17 +94,19 @@ _KINDS = {1.0: 1, 2.0: 2, math.inf: 3}  # norm_type -> PER_NORM_*
 
 
 def _kind(norm_type) -> int:
-    try:
-        return _KINDS[float(norm_type)]
-    except (KeyError, ValueError):
-        raise ValueError(f"norm_type must be 1, 2 or inf, not {norm_type!r}") from None
+    kind = _KINDS.get(norm_type)
+    if kind is None:
+        try:
+            kind = _KINDS[float(norm_type)]
+        except (KeyError, ValueError, TypeError):
+            raise ValueError(f"norm_type must be 1, 2 or inf, not {norm_type!r}") from None
+    return kind
 
 
 def _max_norm(max_norm) -> float:
-    max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
-    return max_norm
+    return max_norm if type(max_norm) is float else float(max_norm)
 
 
 def _listed(tensors) -> list:
