@@ -25,6 +25,13 @@
 // Squares are summed in float32, in 16 sums per thread, and in float64 from
 // there. A CTA whose sum is not finite, or so small that squares may have
 // vanished below the float32 range, sums its run again in float64.
+//
+// DRAM bounds large lists (1.02 GB of bfloat16: 147 us for the norm, 7.0 TB/s
+// read only, 498 us with the scaling, which the 469 us of its three passes at
+// the copy rate bound from below), L2 and the chain of loads and sums the
+// middle (155 MB of float32: norm 26.5 us; 11.4 MB in 100 tensors: 10 us), the
+// launches and the exchange short ones (0.6 MB: 3.8 us in the one kernel, 4.9
+// us in two).
 #include <cuda_runtime.h>
 #include <stdint.h>
 

@@ -11,6 +11,20 @@
 // subtraction in v cancels nothing, and m is known to more than float32's
 // precision; it is kept as the pair (s, avg(d)), because h loses
 // |m| / sqrt(v) units of rounding to a mean held in one float32.
+//
+// Bytes: forward x read and y written once, backward x, dy read and dx written
+// once, plus 16 bytes of statistics a row and the vectors; some 7 and 13
+// operations a value, so that DRAM bounds every size beyond the L2 cache. What
+// a row costs beyond its values (the sums over its threads, addresses, waits)
+// decides how near a kernel comes, so rows are laid out by length (shape_of):
+//   - up to 512 or 1,024 values: LANES threads of a warp, several rows a warp;
+//   - up to 8,192 (backward) and 16,384 (forward) 16-bit values or 8,192
+//     float32 ones: a group of warps, rows copied ahead into shared memory;
+//   - up to eight times that: a cluster of CTAs, each with a slice;
+//   - longer: read from memory in each of two or three passes.
+// The columns' sums dw and db: a thread keeps those of its columns in registers
+// over all its rows; each CTA writes one partial row, and a second kernel adds
+// these in a fixed order, so equal calls give equal bits.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -308,7 +322,10 @@ __device__ __forceinline__ void add_groups(float* part, const float* sums, int g
 }
 
 // ---- short rows: LANES threads of a warp (a power of two) per row, several
-// rows per warp, nothing but shuffles between the threads.
+// rows per warp, nothing but shuffles between the threads. Measured (back to
+// back in a graph, new inputs): 65536x256 float32 24.5 us forward (5.5 TB/s),
+// 35.5 us backward (5.7 TB/s); 8191x1001 half, single values, 12.3 and 19 us; 65536x32 columns of 74-value rows, forward, 7.0
+// us; 1x256 1.25 us, of which the launch is most.
 
 // A thread's own copies on their way into shared memory, STAGES rows ahead:
 // it waits for and reads only what it has copied itself, so no barrier is
@@ -914,6 +931,12 @@ constexpr int kWideThreads = 384;
 template <bool ANY>
 constexpr int kBwdStages = ANY ? 2 : 3;
 
+// Each thread holds its values in registers; two exchanges of the group's warps
+// (mean, then squares) are one, because a warp's own mean and squares are
+// enough to have the row's. Measured: 65536x4096 bfloat16 180 us (6.0 TB/s of
+// the 6.5 TB/s of a copy; 195 us under a second's load, when the clocks fall),
+// 16384x4096 float32 84 us (6.4 TB/s), 8192x16384 float32 in clusters of two
+// 190 us (5.6 TB/s), 20000x1003 float32 35 us (4.6 TB/s).
 template <typename T, typename P, int NV, bool CLUSTER, bool ANY, int THREADS>
 __global__ void __launch_bounds__(THREADS) per_layer_norm_group_kernel(const Fwd f) {
   __shared__ Exchange<CLUSTER> ex;
@@ -1029,6 +1052,11 @@ __global__ void __launch_bounds__(THREADS) per_layer_norm_group_kernel(const Fwd
   if constexpr (CLUSTER) cluster_sync();  // no CTA ends while another may still write to it
 }
 
+// Measured: 65536x4096 bfloat16 250 us (6.4 TB/s), 16384x8192 bfloat16 132 us
+// (6.1 TB/s, 7 us of it the join), 16384x4096 float32 140 us (5.7 TB/s),
+// 8192x16384 float32 in clusters of four 278 us (5.8 TB/s). Rows that start
+// anywhere cost two shifts and a mask more for each vector: 20000x1003 float32
+// 47 us (5.1 TB/s), 9000x5001 bfloat16 104 us (2.6 TB/s).
 // dx, and the column sums of this CTA's rows: each thread keeps the sums of
 // its columns while its group walks down the rows; at the end the groups of a
 // CTA are joined in shared memory and the CTA writes one partial row of dw and
@@ -1115,7 +1143,7 @@ __global__ void __launch_bounds__(kRowThreads) per_layer_norm_backward_group_ker
 }
 
 // ---- rows of any length: one CTA per row, the row read three times (from
-// L2 after the first)
+// L2 after the first). Rows of more than 65,536 to 131,072 values only.
 template <typename T, typename P>
 __global__ void __launch_bounds__(kThreads) per_layer_norm_long_kernel(const Fwd f) {
   per_wait_previous_grid();
@@ -1281,14 +1309,19 @@ struct Shape {
 constexpr int kFwdVectors = 4;
 template <typename T>
 constexpr int kBwdVectors = sizeof(T) == 2 ? 2 : 4;
-constexpr int kSingles = 8;  // of single values, in a warp
+// Single values, in a warp: rows that start anywhere are faster so than by
+// windows as long as a warp can hold them (50000x333 half 21 us against 40
+// forward, 40 against 55 backward; 8191x1001 12 against 15 and 19 against 31;
+// float32 only up to 16 a lane: 20000x1003 backward 54 against 47).
+template <typename T>
+constexpr int kSingles = sizeof(T) == 2 ? 32 : 16;
 
 // Rows that a warp can hold stay in it, which needs no barrier; longer ones
 // take a group of warps, and beyond one CTA a cluster of up to 8. In a warp,
 // rows that start anywhere go by single values (vec 1).
-Shape shape_of(int64_t dim, int vec, bool any, bool split, int full, int most_threads,
+Shape shape_of(int64_t dim, int vec, bool any, bool split, int singles, int full, int most_threads,
                int warp_threads) {
-  const int small = any ? 4 : 1, most = any ? kSingles : full;
+  const int small = any ? 4 : 1, most = any ? singles : full;
   const int64_t w = any ? dim : (dim + vec - 1) / vec;
   for (int lanes = 4; lanes <= 32; lanes *= 2)
     if (w <= lanes * small) return {lanes, small, warp_threads, 1};
@@ -1318,7 +1351,7 @@ Shape shape_of(int64_t dim, int vec, bool any, bool split, int full, int most_th
 #define PER_NORM_SHAPE(s, rc, warp, group, T, P, ANY, FULL, ...)                               \
   [&]() -> bool {                                                                              \
     constexpr int V = ANY ? 1 : 16 / sizeof(T), S = ANY ? 4 : 1, F = FULL;                     \
-    constexpr int W = ANY ? kSingles : F;                                                      \
+    constexpr int W = ANY ? kSingles<T> : F;                                                   \
     if (s.lanes == 4) return rc = warp<T, P, V, S, 4>(s, __VA_ARGS__), true;                   \
     if (s.lanes == 8) return rc = warp<T, P, V, S, 8>(s, __VA_ARGS__), true;                   \
     if (s.lanes == 16) return rc = warp<T, P, V, S, 16>(s, __VA_ARGS__), true;                 \
@@ -1326,7 +1359,10 @@ Shape shape_of(int64_t dim, int vec, bool any, bool split, int full, int most_th
     if (s.lanes == 32 && s.nv == 2 * S)                                                        \
       return rc = warp<T, P, V, 2 * S, 32>(s, __VA_ARGS__), true;                              \
     if constexpr (W >= 4 * S)                                                                  \
-      if (s.lanes == 32) return rc = warp<T, P, V, 4 * S, 32>(s, __VA_ARGS__), true;           \
+      if (s.lanes == 32 && s.nv == 4 * S)                                                      \
+        return rc = warp<T, P, V, 4 * S, 32>(s, __VA_ARGS__), true;                            \
+    if constexpr (W >= 8 * S)                                                                  \
+      if (s.lanes == 32) return rc = warp<T, P, V, 8 * S, 32>(s, __VA_ARGS__), true;           \
     if (s.ctas == 1 && s.nv == F)                                                              \
       return rc = group<T, P, F, false, ANY>(s, __VA_ARGS__), true;                            \
     if (s.ctas == 1) return rc = group<T, P, F / 2, false, ANY>(s, __VA_ARGS__), true;         \
@@ -1384,7 +1420,7 @@ int forward_group(const Shape& s, const Fwd& in, cudaStream_t stream) {
 template <typename T, typename P, bool ANY>
 int forward_rows(const Fwd& f, cudaStream_t stream) {
   constexpr int FULL = kFwdVectors;
-  const Shape s = shape_of(f.dim, 16 / sizeof(T), ANY, true, FULL, kRowThreads, 128);
+  const Shape s = shape_of(f.dim, 16 / sizeof(T), ANY, true, kSingles<T>, FULL, kRowThreads, 128);
   int rc = PER_OK;
   if (PER_NORM_SHAPE(s, rc, forward_warp, forward_group, T, P, ANY, FULL, f, stream)) return rc;
   return launch((const void*)per_layer_norm_long_kernel<T, P>, row_grid(f.rows), kThreads, 0, &f,
@@ -1461,7 +1497,7 @@ int backward_group(const Shape& s, const Bwd& in, cudaStream_t stream) {
 template <typename T, typename P, bool ANY>
 int backward_rows(const Bwd& in, cudaStream_t stream) {
   constexpr int FULL = kBwdVectors<T>;
-  const Shape s = shape_of(in.dim, 16 / sizeof(T), ANY, ANY, FULL, kRowThreads, 256);
+  const Shape s = shape_of(in.dim, 16 / sizeof(T), ANY, ANY, kSingles<T>, FULL, kRowThreads, 256);
   int rc = PER_OK;
   if (PER_NORM_SHAPE(s, rc, backward_warp, backward_group, T, P, ANY, FULL, in, stream)) return rc;
   Bwd g = in;
@@ -1496,7 +1532,7 @@ int64_t backward_bytes(const per_norm_t& n) {
   int64_t most = 0;
   for (const bool any : {false, true}) {
     if (!any && n.dim % VEC) continue;
-    const Shape s = shape_of(n.dim, VEC, any, any, FULL, kRowThreads, 256);
+    const Shape s = shape_of(n.dim, VEC, any, any, kSingles<T>, FULL, kRowThreads, 256);
     const int64_t bytes =
         s.ctas ? most_partials(n.rows, n.dim) * places_of(s, any && s.lanes ? 1 : VEC).padded
                : (int64_t)splits_of(n.rows, n.dim) * long_places((int32_t)n.dim).padded;
