@@ -176,6 +176,43 @@ int per_coresident_clusters(const void* fn, int threads, size_t smem, int cluste
   return PER_OK;
 }
 
+bool per_cluster_fits(const void* fn, int threads, size_t smem, int cluster) {
+  static std::mutex mu;
+  static struct {
+    int device;
+    const void* fn;
+    int cluster;
+    bool fits;
+  } known[512];
+  static int n = 0;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  {
+    std::lock_guard<std::mutex> lk(mu);
+    for (int i = 0; i < n; ++i)
+      if (known[i].device == dev && known[i].fn == fn && known[i].cluster == cluster)
+        return known[i].fits;
+  }
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = cluster;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(cluster);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int clusters = 0;
+  const bool fits =
+      cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+      cudaOccupancyMaxActiveClusters(&clusters, fn, &cfg) == cudaSuccess && clusters > 0;
+  if (!fits) cudaGetLastError();  // not an error of this call: another kernel serves it
+  std::lock_guard<std::mutex> lk(mu);
+  if (n < 512) known[n++] = {dev, fn, cluster, fits};
+  return fits;
+}
+
 int per_set_smem(const void* fn, size_t smem) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);

@@ -35,8 +35,6 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
-#include <mutex>
-
 #include "per_common.cuh"
 #include "per_internal.h"
 #include "per_types.cuh"
@@ -615,39 +613,6 @@ const void* short_kernel(int32_t kind) {
                                : (const void*)per_clip_short_kernel<T, PER_NORM_INF>;
 }
 
-// Whether the current device runs clusters of kCluster CTAs of `fn` (more than
-// the 8 that every device of this architecture does); asked once per device.
-bool cluster_fits(const void* fn) {
-  static std::mutex mu;
-  static struct {
-    int device;
-    const void* fn;
-    bool fits;
-  } known[64];
-  static int n = 0;
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return false;
-  std::lock_guard<std::mutex> lk(mu);
-  for (int i = 0; i < n; ++i)
-    if (known[i].device == dev && known[i].fn == fn) return known[i].fits;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = kCluster;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(kCluster);
-  cfg.blockDim = dim3(kThreads);
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  int clusters = 0;
-  const bool fits =
-      cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
-      cudaOccupancyMaxActiveClusters(&clusters, fn, &cfg) == cudaSuccess && clusters > 0;
-  if (!fits) cudaGetLastError();  // not an error of this call: another kernel serves it
-  if (n < 64) known[n++] = {dev, fn, fits};
-  return fits;
-}
-
 // One kernel for up to a megabyte of one type; false where the list is another.
 bool one_kernel(const per_tensor_t* list, int64_t n, const Call& c, bool scaling,
                 cudaStream_t stream, int* rc) {
@@ -675,7 +640,7 @@ bool one_kernel(const per_tensor_t* list, int64_t n, const Call& c, bool scaling
   const void* fn = dtype == PER_F32    ? short_kernel<float>(c.kind)
                    : dtype == PER_BF16 ? short_kernel<__nv_bfloat16>(c.kind)
                                        : short_kernel<__half>(c.kind);
-  if (!cluster_fits(fn)) return false;
+  if (!per_cluster_fits(fn, kThreads, 0, kCluster)) return false;
   void* args[] = {&t};
   const cudaError_t e = per_launch_cluster(fn, kCluster, kThreads, 0, kCluster, stream, args);
   *rc = e == cudaSuccess ? PER_OK : per_record_cuda(e);

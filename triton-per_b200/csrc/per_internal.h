@@ -34,6 +34,11 @@ int per_coresident_ctas(const void* fn, int threads, size_t smem, int* out);
 // GPU's processing clusters.
 int per_coresident_clusters(const void* fn, int threads, size_t smem, int cluster, int* out);
 
+// Whether the current device runs clusters of up to 16 CTAs of `fn` (8 is what
+// every device of this architecture does, 16 has to be asked for); cached per
+// (device, fn, cluster).
+bool per_cluster_fits(const void* fn, int threads, size_t smem, int cluster);
+
 // Allow `fn` to use up to `smem` bytes of dynamic shared memory on the
 // current device (needed whenever static + dynamic exceeds 48 KB); cached per
 // (device, fn).

@@ -60,6 +60,7 @@ struct Bwd {
   int64_t rows, dy_stride, x_stride, dx_stride;
   int32_t dim, splits;
   int32_t group_threads;  // of a row that spans warps
+  int32_t joined;         // one cluster: no partial rows, its CTAs add their sums themselves
   struct Places {         // the order of the columns in a partial row, see store_columns()
     int32_t padded, slice, width, vec;
   } places;
@@ -321,6 +322,31 @@ __device__ __forceinline__ void add_groups(float* part, const float* sums, int g
   }
 }
 
+// ---- clusters of CTAs
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ uint32_t remote_address(const void* p, uint32_t cta) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+               : "=r"(r)
+               : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(cta));
+  return r;
+}
+
 // ---- short rows: LANES threads of a warp (a power of two) per row, several
 // rows per warp, nothing but shuffles between the threads. Measured (back to
 // back in a graph, new inputs): 65536x256 float32 24.5 us forward (5.5 TB/s),
@@ -434,6 +460,8 @@ __global__ void __launch_bounds__(128) per_layer_norm_warp_kernel(const Fwd f) {
   }
 }
 
+constexpr int kJoinCtas = 16;  // of a launch that joins its own column sums
+
 // Rows beyond the last read as dy = 0 and so add nothing to any sum.
 template <typename T, typename P, int VEC, int NV, int LANES>
 __global__ void __launch_bounds__(256) per_layer_norm_backward_warp_kernel(const Bwd g) {
@@ -500,7 +528,7 @@ __global__ void __launch_bounds__(256) per_layer_norm_backward_warp_kernel(const
       store_row(static_cast<T*>(g.dx) + row * g.dx_stride, o, lane, LANES, g.dim);
     }
   }
-  if (!g.part) return;
+  if (!g.part && !g.joined) return;
   // the row groups of a warp by shuffles, then the warps through shared
   // memory, where the (empty) copies still in flight have ended
   constexpr int kPadded = LANES * NV * VEC;
@@ -522,7 +550,31 @@ __global__ void __launch_bounds__(256) per_layer_norm_backward_warp_kernel(const
     store_columns<VEC, NV>(own + kPadded, ab, lane, LANES);
   }
   __syncthreads();
-  add_groups(g.part + (int64_t)blockIdx.x * 2 * kPadded, sums, blockDim.x >> 5, kPadded);
+  if (!g.joined) {
+    add_groups(g.part + (int64_t)blockIdx.x * 2 * kPadded, sums, blockDim.x >> 5, kPadded);
+    return;
+  }
+  // Few rows: the launch is one cluster, and each of its CTAs adds a share of the columns over all.
+  float* all = sums + (blockDim.x >> 5) * 2 * kPadded;
+  add_groups(all, sums, blockDim.x >> 5, kPadded);
+  cluster_sync();
+  const int ctas = (int)cluster_size();
+  for (int p = (int)(cluster_rank() * blockDim.x + threadIdx.x); p < 2 * kPadded; p += ctas * blockDim.x) {
+    float u[kJoinCtas];
+#pragma unroll
+    for (int c = 0; c < kJoinCtas; ++c) {  // every load on its way before the first is needed
+      u[c] = 0.f;
+      if (c < ctas)
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(u[c]) : "r"(remote_address(all + p, c)));
+    }
+    float v = 0.f;
+#pragma unroll
+    for (int c = 0; c < kJoinCtas; ++c) v += u[c];
+    const int c = column_at(g.places, p % kPadded);
+    void* out = p < kPadded ? g.dw : g.db;
+    if (out && c < g.dim) static_cast<P*>(out)[c] = per_from_f32<P>(v);
+  }
+  cluster_sync();  // no CTA ends while another may still read from it
 }
 
 // ---- longer rows: a group of warps per row (several groups in a CTA), or a
@@ -531,22 +583,6 @@ __global__ void __launch_bounds__(256) per_layer_norm_backward_warp_kernel(const
 constexpr int kMaxCluster = 8;
 constexpr int kRowThreads = 512;  // of a CTA
 constexpr int kMaxGroups = 8;
-
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t cluster_size() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  __syncwarp();
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 
 // A thread's place: `lane` of `width` threads that hold the values first ..
 // first + dim of a row.
@@ -593,14 +629,6 @@ struct Exchange {
   float4 slot[2][kWarps];
   uint64_t arrived[2];  // CLUSTER
 };
-
-__device__ __forceinline__ uint32_t remote_address(const void* p, uint32_t cta) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
-               : "=r"(r)
-               : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(cta));
-  return r;
-}
 
 // The state of a thread in the exchanges of its row.
 template <bool CLUSTER>
@@ -1474,8 +1502,25 @@ int backward_warp(const Shape& s, const Bwd& in, cudaStream_t stream) {
   g.places = places_of(s, VEC);
   const size_t ring = Ring<T, VEC, 2 * NV, kWarpStages>::kBytes * s.threads;
   const size_t sums = (size_t)(s.threads / 32) * 2 * g.places.padded * 4;
-  return backward_run<P>((const void*)per_layer_norm_backward_warp_kernel<T, P, VEC, NV, LANES>, s,
-                         s.threads, ring > sums ? ring : sums, g, stream);
+  const void* fn = (const void*)per_layer_norm_backward_warp_kernel<T, P, VEC, NV, LANES>;
+  // Few rows (up to two turns of 16 CTAs): one launch, a cluster that joins its
+  // own sums. In an eager step that saves 2 us of host time (256x256 float32: 62
+  // to 60 us); longer ones would wait longer for 16 CTAs than a launch takes.
+  const int64_t turn = s.threads / LANES;
+  const size_t joined = sums + (size_t)2 * g.places.padded * 4;
+  if ((g.dw || g.db) && g.rows <= 2 * kJoinCtas * turn && joined <= 100 * 1024) {
+    int ctas = 1;
+    while (ctas < kJoinCtas && ctas * turn < g.rows) ctas *= 2;
+    const size_t smem = ring > joined ? ring : joined;
+    const int rc = per_set_smem(fn, smem);
+    if (rc) return rc;
+    if (ctas <= 8 || per_cluster_fits(fn, s.threads, smem, ctas)) {
+      g.joined = 1;
+      g.part = nullptr;
+      return launch(fn, ctas, s.threads, smem, &g, stream, ctas);
+    }
+  }
+  return backward_run<P>(fn, s, s.threads, ring > sums ? ring : sums, g, stream);
 }
 
 template <typename T, typename P, int NV, bool CLUSTER, bool ANY>
@@ -1570,6 +1615,6 @@ int per_launch_layer_norm_backward(const per_norm_t& n, const void* dy, int64_t 
                                    cudaStream_t stream) {
   const Bwd g{dy, x, weight, reinterpret_cast<const float4*>(stats), dx, dweight, dbias,
               static_cast<float*>(workspace),
-              n.rows, dy_stride, x_stride, dx_stride, (int32_t)n.dim, 0, 0, {}};
+              n.rows, dy_stride, x_stride, dx_stride, (int32_t)n.dim, 0, 0, 0, {}};
   return PER_NORM_TYPES(n, backward, g, stream);
 }
