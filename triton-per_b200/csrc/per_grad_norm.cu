@@ -270,13 +270,13 @@ __device__ __forceinline__ void sum_fetched(W& w, const uint4 (&u)[K], S& acc) {
     }
 }
 
-// A CTA's run into `acc`.
+// A CTA's run into `acc`. The walk over it is the caller's, who can have found
+// its way through the list before there is anything to read.
 template <typename TB, typename S>
-__device__ __forceinline__ void sum_run(const TB& t, S& acc) {
+__device__ __forceinline__ void sum_run(const TB& t, Walk<TB, 1> w, S& acc) {
   for_loose(t, [&](char* p, int dtype) {
     with_type(dtype, [&](auto z) { acc.add(*reinterpret_cast<const decltype(z)*>(p)); });
   });
-  Walk<TB, 1> w(t);
   while (w.more) {
     if (w.left() >= kUnroll) {  // blocks of one tensor
       const int64_t blocks = w.left() / kUnroll * kUnroll;
@@ -325,13 +325,14 @@ __device__ __forceinline__ double block_join(double v, bool take_max) {
 template <typename TB, int KIND>
 __global__ void __launch_bounds__(kThreads, 2)
     per_norm_partial_kernel(const __grid_constant__ TB t) {
+  const Walk<TB, 1> w(t);
   per_wait_previous_grid();
   Sums<KIND> acc;
-  sum_run(t, acc);
+  sum_run(t, w, acc);
   double sum = block_join(acc.total(), KIND == PER_NORM_INF);
   if (leaves_float32(sum, KIND)) {
     WideSum<KIND> wide;
-    sum_run(t, wide);
+    sum_run(t, Walk<TB, 1>(t), wide);
     sum = block_join(wide.s, false);
   }
   if (threadIdx.x == 0) t.part[t.first_partial + blockIdx.x] = sum;

@@ -6,8 +6,9 @@ norm. These are drop-ins for torch.nn.functional.layer_norm, torch.nn.LayerNorm
 and torch.nn.utils.clip_grad_norm_ / get_total_norm / clip_grads_with_norm_ on
 CUDA tensors of float32, bfloat16 or float16. Every call enqueues its work on
 the current stream of the tensors' device, synchronises nothing (except
-error_if_nonfinite=True) and can be captured into a CUDA graph. As with the
-buffers there is no CPU path.
+error_if_nonfinite=True) and can be captured into a CUDA graph. Tensors made on
+another stream are the caller's to order, as for torch's own operators
+(wait_stream, record_stream). As with the buffers there is no CPU path.
 """
 
 from __future__ import annotations
@@ -118,7 +119,7 @@ def _listed(tensors) -> list:
 def grad_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
     """The norm of all values of `tensors` (a tensor or an iterable of them,
     of mixed types, on one device) as one vector: a float32 scalar on their
-    device. norm_type is 1, 2 or inf."""
+    device, not differentiable. norm_type is 1, 2 or inf."""
     kind = _kind(norm_type)
     norm = _binding().grad_norm(_listed(tensors), False, kind)
     return torch.tensor(0.0) if norm is None else norm
