@@ -28,6 +28,7 @@ NVCC_FLAGS = [
     "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "-Xcompiler", "-O2",
     "-shared", "-cudart", "static",
+    "--threads", "0",  # the sources in parallel
 ]
 
 
