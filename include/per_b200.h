@@ -315,10 +315,9 @@ int per_update_priorities_shard_count(const per_store_t* store, int64_t base, co
                                       void* stream);
 
 /* ---- operators of the learner that trains on the sampled batches (no
- * counterpart in the reference's library; its learner,
- * experiments/sac.py, takes them from PyTorch). A step runs them between
- * sample and update_priorities: layer norm in the networks, forward and
- * backward, then the clipping of all gradients by their global norm. */
+ * counterpart in the reference). A step runs them between sample and
+ * update_priorities: layer norm in the networks, forward and backward, then
+ * the clipping of all gradients by their global norm. */
 
 /* element types */
 #define PER_F32 0
@@ -385,7 +384,8 @@ int64_t per_grad_norm_workspace(int64_t n);
 /* *norm = the norm of all values of all tensors (float32 on the device): the
  * root of the sum of squares, the sum of absolute values, or the largest one.
  * NaN where a value is NaN. Values whose squares leave the float32 range are
- * summed in float64. `tensors` is a host array, read during the call only.
+ * summed in float64. `tensors` is a host array, read during the call only;
+ * `norm` must not be part of a tensor or of the workspace.
  * Workspace as in per_layer_norm_backward(). */
 int per_grad_norm(const per_tensor_t* tensors, int64_t n, int32_t kind, float* norm,
                   void* workspace, int64_t workspace_bytes, void* stream);
@@ -393,7 +393,8 @@ int per_grad_norm(const per_tensor_t* tensors, int64_t n, int32_t kind, float* n
 /* Multiply every value by min(1, max_norm / (*norm + 1e-6)), in float32 and
  * rounded once; tensors are not touched where that factor is 1. `norm` is a
  * device float32 (of per_grad_norm(), or joined over the ranks of a job). The
- * factor is NaN where *norm is NaN, and 0 where it is infinite. No two tensors
+ * factor is NaN where *norm is NaN (or both norms are infinite), and 0 where
+ * *norm alone is infinite. No two tensors
  * may overlap, nor may *norm be part of one. */
 int per_scale_grads(const per_tensor_t* tensors, int64_t n, float max_norm, const float* norm,
                     void* stream);
