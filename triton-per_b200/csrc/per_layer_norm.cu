@@ -945,7 +945,15 @@ struct Outbox {
   }
 };
 
-constexpr int kFwdStages = 3;
+// Rows ahead, of which more cost shared memory that nothing else needs: two
+// are enough for the forward pass (16384x8192 bfloat16 93 us, three: 99) and for
+// float32 rows backward (8192x16384: 238 us, three: 280); 16-bit rows backward,
+// half the bytes, take three (16384x8192: 133 us, two: 146), unless an outbox
+// has to fit beside them.
+constexpr int kFwdStages = 2;
+template <typename T, bool ANY>
+constexpr int kBwdStages = ANY || sizeof(T) == 4 ? 2 : 3;
+
 // Threads that a CTA is compiled for, which bounds a thread's registers. 32
 // values of 16-bit rows with their weights and biases take some 144: CTAs of
 // up to 192 threads get them (168 each, and as many CTAs per SM), since what
@@ -955,16 +963,13 @@ constexpr int kFwdStages = 3;
 template <typename T, int NV>
 constexpr bool kWide = sizeof(T) == 2 && NV == 4;
 constexpr int kWideThreads = 384;
-// Three rows ahead; two where an outbox has to fit beside them.
-template <bool ANY>
-constexpr int kBwdStages = ANY ? 2 : 3;
 
 // Each thread holds its values in registers; two exchanges of the group's warps
 // (mean, then squares) are one, because a warp's own mean and squares are
-// enough to have the row's. Measured: 65536x4096 bfloat16 180 us (6.0 TB/s of
-// the 6.5 TB/s of a copy; 195 us under a second's load, when the clocks fall),
-// 16384x4096 float32 84 us (6.4 TB/s), 8192x16384 float32 in clusters of two
-// 190 us (5.6 TB/s), 20000x1003 float32 35 us (4.6 TB/s).
+// enough to have the row's. Measured: 65536x4096 bfloat16 177 us (6.1 TB/s of
+// the 6.5 TB/s of a copy; 193 us under a second's load, when the clocks fall),
+// 16384x4096 float32 83 us (6.4 TB/s), 8192x16384 float32 in clusters of two
+// 189 us (5.6 TB/s), 20000x1003 float32 34-37 us (4.4-4.7 TB/s).
 template <typename T, typename P, int NV, bool CLUSTER, bool ANY, int THREADS>
 __global__ void __launch_bounds__(THREADS) per_layer_norm_group_kernel(const Fwd f) {
   __shared__ Exchange<CLUSTER> ex;
@@ -1081,17 +1086,17 @@ __global__ void __launch_bounds__(THREADS) per_layer_norm_group_kernel(const Fwd
 }
 
 // Measured: 65536x4096 bfloat16 250 us (6.4 TB/s), 16384x8192 bfloat16 132 us
-// (6.1 TB/s, 7 us of it the join), 16384x4096 float32 140 us (5.7 TB/s),
-// 8192x16384 float32 in clusters of four 278 us (5.8 TB/s). Rows that start
+// (6.1 TB/s, 7 us of it the join), 16384x4096 float32 135 us (6.0 TB/s),
+// 8192x16384 float32 in clusters of two 238 us (6.8 TB/s). Rows that start
 // anywhere cost two shifts and a mask more for each vector: 20000x1003 float32
-// 47 us (5.1 TB/s), 9000x5001 bfloat16 104 us (2.6 TB/s).
+// 47-49 us (4.9-5.1 TB/s), 9000x5001 bfloat16 104 us (2.6 TB/s).
 // dx, and the column sums of this CTA's rows: each thread keeps the sums of
 // its columns while its group walks down the rows; at the end the groups of a
 // CTA are joined in shared memory and the CTA writes one partial row of dw and
 // db. Columns beyond the row read as dy = 0 and so add nothing to any sum.
 template <typename T, typename P, int NV, bool CLUSTER, bool ANY>
 __global__ void __launch_bounds__(kRowThreads) per_layer_norm_backward_group_kernel(const Bwd g) {
-  constexpr int VEC = 16 / sizeof(T), kStages = kBwdStages<ANY>;
+  constexpr int VEC = 16 / sizeof(T), kStages = kBwdStages<T, ANY>;
   __shared__ Exchange<CLUSTER> ex;
   __shared__ __align__(8) uint64_t bars[kMaxGroups][kStages];
   extern __shared__ __align__(16) unsigned char dyn[];
@@ -1530,7 +1535,7 @@ int backward_group(const Shape& s, const Bwd& in, cudaStream_t stream) {
   // several groups share a CTA and its partial row
   int groups = CLUSTER ? 1 : kRowThreads / s.threads;
   groups = groups > kMaxGroups ? kMaxGroups : groups;
-  size_t smem = groups * (Rows<T, NV, 2, kBwdStages<ANY>, true, ANY>::bytes(s.threads) +
+  size_t smem = groups * (Rows<T, NV, 2, kBwdStages<T, ANY>, true, ANY>::bytes(s.threads) +
                           (ANY ? Outbox<T, NV>::bytes(s.threads) : 0));
   g.places = places_of(s, 16 / sizeof(T));
   const size_t sums = groups > 1 ? (size_t)groups * 2 * g.places.padded * 4 : 0;
