@@ -437,6 +437,31 @@ def test_second_derivative_is_refused():
         torch.autograd.grad(y.square().sum(), x, create_graph=True)
 
 
+def test_forward_mode_is_refused():
+    x, w = normal(4, 8), torch.ones(8, device="cuda")
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            per_b200.layer_norm(dual, 8)
+        dual = torch.autograd.forward_ad.make_dual(w, torch.ones_like(w))
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            per_b200.layer_norm(x, 8, dual, w)
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            per_b200.layer_norm(x, 8, w, dual)
+
+
+def test_lazily_negated_views():
+    x, w, b, dy = normal(6, 40), normal(40), normal(40), normal(6, 40)
+    neg = [torch._neg_view(t.neg()) for t in (x, w, b, dy)]  # the same values, negated when read
+    assert all(t.is_neg() for t in neg)
+    check_forward(neg[0], neg[1], neg[2])
+    leaves = [t.detach().requires_grad_() for t in neg[:3]]
+    got = torch.autograd.grad(per_b200.layer_norm(leaves[0], 40, *leaves[1:]), leaves, neg[3])
+    leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+    want = torch.autograd.grad(per_b200.layer_norm(leaves[0], 40, *leaves[1:]), leaves, dy)
+    assert all(torch.equal(g, h) for g, h in zip(got, want))  # the same calls on copies
+
+
 def test_second_backward_and_changed_inputs_are_refused():
     x = normal(4, 8).requires_grad_()
     y = per_b200.layer_norm(x, 8)

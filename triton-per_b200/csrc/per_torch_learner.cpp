@@ -93,6 +93,10 @@ std::pair<Tensor, int64_t> rows_of(const Tensor& t, int64_t norm_dims, int64_t d
   return {t.contiguous(), dim};
 }
 
+// The values in memory: a lazily negated view (the imaginary part of a
+// conjugated tensor) holds them with the other sign.
+Tensor plain(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+
 void* ptr_or_null(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 struct Shape {
@@ -122,8 +126,8 @@ struct LayerNormBackward : public torch::autograd::Node {
     TORCH_CHECK(!at::GradMode::is_enabled(),
                 "per_b200.layer_norm: its gradient is not differentiable again "
                 "(backward with create_graph=True)");
-    const Tensor xv = x.unpack();
-    const Tensor wv = has_weight ? weight.unpack().contiguous() : Tensor();
+    const Tensor xv = plain(x.unpack());
+    const Tensor wv = has_weight ? plain(weight.unpack()).contiguous() : Tensor();
     const bool want_x = task_should_compute_output(0);
     const bool want_w = has_weight && task_should_compute_output(1);
     const bool want_b = has_bias && task_should_compute_output(2);
@@ -131,7 +135,7 @@ struct LayerNormBackward : public torch::autograd::Node {
     TORCH_CHECK(grads[0].device() == xv.device() && grads[0].scalar_type() == xv.scalar_type(),
                 "per_b200.layer_norm: the gradient must have the input's type and device");
     const auto [xr, xs] = rows_of(xv, shape.norm_dims, shape.dim);
-    const auto [dy, ds] = rows_of(grads[0], shape.norm_dims, shape.dim, true);
+    const auto [dy, ds] = rows_of(plain(grads[0]), shape.norm_dims, shape.dim, true);
     if (want_x) out[0] = fresh(xv.sizes(), xv.scalar_type(), xv.device());
     const auto norm_sizes = xv.sizes().slice(xv.dim() - shape.norm_dims);
     if (want_w) out[1] = fresh(norm_sizes, param_type, xv.device());
@@ -192,6 +196,9 @@ Tensor layer_norm(const Tensor& x, const std::vector<int64_t>& normalized_shape,
   for (int64_t d = 0; d < lead; ++d) s.rows *= x.size(d);
   if (!(eps >= 0)) throw py::value_error("layer_norm: eps must not be negative");
   Tensor w = weight ? *weight : Tensor(), b = bias ? *bias : Tensor();
+  for (const Tensor* t : {&x, static_cast<const Tensor*>(&w), static_cast<const Tensor*>(&b)})
+    if (t->defined() && t->_fw_grad(0).defined())
+      throw std::runtime_error("per_b200.layer_norm has no forward-mode derivative");
   at::ScalarType param_type = at::kFloat;
   for (const Tensor* p : {&w, &b}) {
     if (!p->defined()) continue;
@@ -224,11 +231,12 @@ Tensor layer_norm(const Tensor& x, const std::vector<int64_t>& normalized_shape,
   {
     at::AutoDispatchBelowADInplaceOrView below;
     int64_t xs = 0;
-    std::tie(xr, xs) = rows_of(x, s.norm_dims, s.dim);
+    std::tie(xr, xs) = rows_of(plain(x), s.norm_dims, s.dim);
     y = fresh(x.sizes(), x.scalar_type(), x.device());
     if (grad) stats = fresh({s.rows, 4}, at::kFloat, x.device());
     if (s.rows > 0 && s.dim > 0) {
-      const Tensor wc = w.defined() ? w.contiguous() : w, bc = b.defined() ? b.contiguous() : b;
+      const Tensor wc = w.defined() ? plain(w).contiguous() : w;
+      const Tensor bc = b.defined() ? plain(b).contiguous() : b;
       const per_norm_t n{s.rows, s.dim, code_of(x.scalar_type()), code_of(param_type), (float)eps};
       check("per_layer_norm",
             per_layer_norm(&n, xr.data_ptr(), xs, ptr_or_null(wc), ptr_or_null(bc), y.data_ptr(),

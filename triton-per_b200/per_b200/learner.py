@@ -37,7 +37,7 @@ def _binding():
 def layer_norm(input: torch.Tensor, normalized_shape, weight: torch.Tensor | None = None,
                bias: torch.Tensor | None = None, eps: float = 1e-5) -> torch.Tensor:
     """Layer norm over the trailing dimensions `normalized_shape`, as
-    torch.nn.functional.layer_norm; differentiable once.
+    torch.nn.functional.layer_norm; differentiable once, in reverse mode.
 
     The result has the input's type and is contiguous; weight and bias are
     float32 or of the input's type (under autocast the types stay as they
