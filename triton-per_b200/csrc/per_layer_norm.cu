@@ -773,14 +773,17 @@ __device__ __forceinline__ uint4 window(const unsigned char* base, int i, int ph
 // The rows of a group on their way into shared memory, STAGES of them, ARRAYS
 // arrays each (plus, STATS, the 16 bytes of a row's statistics), by bulk copies
 // that one thread issues, so that the others spend no instruction on
-// addresses. A slot is filled again once a barrier of the group has followed
-// its reading.
+// addresses. A slot is filled again once every thread of the group is known to
+// have read it: each has put what it read into the exchange that precedes.
 //
 // ANY false: rows are whole vectors on 16-byte boundaries. ANY: rows of any
 // length that start anywhere; the copy takes the 16-byte blocks that hold a row
 // (its neighbours' values come along and are masked), except where such a block
 // would reach beyond the array, before its first row or behind its last: those
-// rows are fetched value by value.
+// rows are fetched value by value, by ordinary stores of all threads, which only
+// a barrier orders before other threads' reads (and the Outbox's reads before
+// its next row). Within one CTA the exchange has one; the st.async of a cluster's
+// exchange orders nothing but its own bytes, so there the kernels add one.
 template <typename T, int NV, int ARRAYS, int STAGES, bool STATS, bool ANY>
 struct Rows {
   static constexpr int VEC = 16 / sizeof(T);
@@ -1052,6 +1055,7 @@ __global__ void __launch_bounds__(THREADS) per_layer_norm_group_kernel(const Fwd
     const float e1 = lanes_sum<32>(e.x), e2 = lanes_sum<32>(e.y);
     const float u = over(e1, own, inv_own);
     put(ex, turns, t, make_float4(s, u, fmaxf(fmaf(-e1, u, e2), 0.f), 0.f));
+    if constexpr (CLUSTER && ANY) cta_part_sync(t);  // see Rows
     fetch(rows.stage, row + kFwdStages * t.step);
     const float s0 = ex.slot[turns.turn][all.from].x;
     float z = 0.f, sq = 0.f, zq[Q];
@@ -1145,6 +1149,7 @@ __global__ void __launch_bounds__(kRowThreads) per_layer_norm_backward_group_ker
       e = backward_sums(qx, qy, w, st.x, st.y, r, h, gv, aw, ab);
     }
     const float v = exchange_split(ex, turns, t, span, lanes_sum_split<32>(e.x, e.y));
+    if constexpr (CLUSTER && ANY) cta_part_sync(t);  // see Rows
     fetch(rows.stage, row + kStages * t.step);
     if (g.dx) {
       Pack<T, VEC> o[NV];
