@@ -5,6 +5,8 @@
 // share none) and calls the C ABI. No kernels here.
 #include <torch/extension.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/function.h>
@@ -52,6 +54,40 @@ void* stream_of(const Tensor& t) {
 // 1 us of host time less than at::empty, of which a training step makes six).
 Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, c10::Device device) {
   return Tensor(at::detail::empty_cuda(sizes, type, device, std::nullopt));
+}
+
+// A tracer records what the dispatcher sees, and these calls pass beneath it:
+// their results would go into the trace as constants. Refused while one is at
+// work: torch.jit.trace (and ONNX export by it), make_fx, fake tensors,
+// functionalization, torch.export. Other dispatch modes (counters, selective
+// recomputation) change no result by not seeing the call.
+bool being_traced() {
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  using Key = c10::impl::TorchDispatchModeKey;
+  using D = c10::DispatchKey;
+  constexpr c10::DispatchKeySet tracers({D::Tracer, D::PreDispatch}), modes(D::Python);
+  const c10::DispatchKeySet tls = c10::impl::tls_local_dispatch_key_set().included_;
+  if (C10_LIKELY(!tls.has_any(tracers | modes))) return false;
+  return tls.has_any(tracers) ||
+         (Modes::get_mode(Key::PROXY) || Modes::get_mode(Key::FAKE) || Modes::get_mode(Key::FUNCTIONAL));
+}
+
+void refuse_tracing(const char* what) {
+  if (being_traced())
+    throw std::runtime_error(std::string("per_b200.") + what +
+                             " cannot be traced or exported (its result would be recorded as a "
+                             "constant); use torch's own operator in what is traced");
+}
+
+// Tensors of vmap, torch.func and functionalization have no memory of their own.
+void refuse_wrapped(const Tensor& t, const char* what) {
+  using D = c10::DispatchKey;
+  constexpr c10::DispatchKeySet wrappers(
+      {D::FuncTorchBatched, D::BatchedNestedTensor, D::FuncTorchGradWrapper, D::Functionalize});
+  if (C10_UNLIKELY(t.key_set().has_any(wrappers)))
+    throw std::runtime_error(std::string("per_b200.") + what +
+                             " takes plain tensors only (it cannot be used under vmap, torch.func "
+                             "transforms or functionalization)");
 }
 
 // ------------------------------------------------------------- layer norm
@@ -123,6 +159,7 @@ struct LayerNormBackward : public torch::autograd::Node {
     std::lock_guard<std::mutex> lock(mutex_);
     torch::autograd::variable_list out(3);
     if (grads.empty() || !grads[0].defined()) return out;
+    TORCH_CHECK(!being_traced(), "per_b200.layer_norm: its backward pass cannot be traced");
     TORCH_CHECK(!at::GradMode::is_enabled(),
                 "per_b200.layer_norm: its gradient is not differentiable again "
                 "(backward with create_graph=True)");
@@ -176,6 +213,7 @@ void check_capture(const Tensor& t, const char* name) {
 Tensor layer_norm(const Tensor& x, const std::vector<int64_t>& normalized_shape,
                   const std::optional<Tensor>& weight, const std::optional<Tensor>& bias,
                   double eps) {
+  refuse_tracing("layer_norm");
   if (!x.is_cuda())
     throw std::runtime_error("per_b200.layer_norm runs on CUDA devices only (no CPU fallback)");
   if (x.layout() != at::kStrided) throw py::type_error("layer_norm: input must be strided");
@@ -196,9 +234,12 @@ Tensor layer_norm(const Tensor& x, const std::vector<int64_t>& normalized_shape,
   for (int64_t d = 0; d < lead; ++d) s.rows *= x.size(d);
   if (!(eps >= 0)) throw py::value_error("layer_norm: eps must not be negative");
   Tensor w = weight ? *weight : Tensor(), b = bias ? *bias : Tensor();
-  for (const Tensor* t : {&x, static_cast<const Tensor*>(&w), static_cast<const Tensor*>(&b)})
-    if (t->defined() && t->_fw_grad(0).defined())
+  for (const Tensor* t : {&x, static_cast<const Tensor*>(&w), static_cast<const Tensor*>(&b)}) {
+    if (!t->defined()) continue;
+    refuse_wrapped(*t, "layer_norm");
+    if (t->_fw_grad(0).defined())
       throw std::runtime_error("per_b200.layer_norm has no forward-mode derivative");
+  }
   at::ScalarType param_type = at::kFloat;
   for (const Tensor* p : {&w, &b}) {
     if (!p->defined()) continue;
@@ -277,6 +318,7 @@ struct List {
                                " runs on CUDA devices only (no CPU fallback)");
     if (g.layout() != at::kStrided)
       throw py::type_error(std::string(what) + ": gradients must be strided (dense) tensors");
+    refuse_wrapped(g, what);
     const int32_t code = code_of(g.scalar_type());
     if (code < 0)
       throw py::type_error(std::string(what) + ": gradients must be float32, bfloat16 or float16");
@@ -318,6 +360,7 @@ struct List {
 };
 
 List list_of(const py::list& tensors, bool take_grads, const char* what) {
+  refuse_tracing(what);
   List l;
   l.impl.reserve(tensors.size());
   l.t.reserve(tensors.size());

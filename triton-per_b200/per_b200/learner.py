@@ -9,6 +9,11 @@ the current stream of the tensors' device, synchronises nothing (except
 error_if_nonfinite=True) and can be captured into a CUDA graph. Tensors made on
 another stream are the caller's to order, as for torch's own operators
 (wait_stream, record_stream). As with the buffers there is no CPU path.
+
+The calls are no torch operators, so nothing that records or transforms
+operators sees them: torch.jit.trace, ONNX export, make_fx, torch.export, fake
+tensors, vmap and the torch.func transforms are refused, and torch.compile
+breaks its graph at each call (fullgraph=True raises).
 """
 
 from __future__ import annotations
