@@ -66,23 +66,20 @@ struct Bwd {
   } places;
 };
 
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(PER_FULL_MASK, v, o);
-  return v;
-}
-
 // Sums of a and b over the CTA, in a fixed order; every thread gets them.
-__device__ __forceinline__ float2 block_sum2(float a, float b) {
-  __shared__ float2 s[32];
-  a = warp_sum(a);
-  b = warp_sum(b);
+__device__ __forceinline__ double2 block_sum2(double a, double b) {
+  __shared__ double2 s[32];
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    a += __shfl_xor_sync(PER_FULL_MASK, a, o);
+    b += __shfl_xor_sync(PER_FULL_MASK, b, o);
+  }
   __syncthreads();  // the previous sums have been read
-  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = make_float2(a, b);
+  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = make_double2(a, b);
   __syncthreads();
-  const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
-  const float2 v = lane < warps ? s[lane] : make_float2(0.f, 0.f);
-  return make_float2(warp_sum(v.x), warp_sum(v.y));
+  double2 v = s[0];
+  for (int k = 1; k < (int)(blockDim.x >> 5); ++k) v.x += s[k].x, v.y += s[k].y;
+  return v;
 }
 
 // a / n for a count n, with inv = 1 / n: the first quotient corrected by its
@@ -1181,28 +1178,55 @@ __global__ void __launch_bounds__(kRowThreads) per_layer_norm_backward_group_ker
 }
 
 // ---- rows of any length: one CTA per row, the row read three times (from
-// L2 after the first). Rows of more than 65,536 to 131,072 values only.
+// L2 after the first). Rows of more than 65,536 to 131,072 values only. The
+// loads of single values in flight bound it, so the launch bounds ask for the
+// registers of 6 and 8 CTAs an SM (3000x303201 float32 forward 3.79 ms, with 5
+// CTAs 4.38; 1000x140001 half backward 0.72 ms, with 6 CTAs 1.02). 512x200000
+// float32: 566 us forward (1.4 TB/s), 914 us backward (1.3 TB/s); a single row
+// of a million takes 1.2 ms, for which one CTA has no more loads to offer.
+
+// Sums of f(i) = (a, b) over i = first, first + step, ... below end. A sum of
+// millions of terms in float32 rounds each of them to the sum's own step (a row
+// of 2^27 equal squares came out 0.7 % off), so float32 takes kRun terms at a
+// time and float64 the rest.
+constexpr int kRun = 32;
+template <typename F>
+__device__ __forceinline__ double2 long_sums(int64_t first, int64_t step, int64_t end, F f) {
+  double2 sum = make_double2(0.0, 0.0);
+  int64_t i = first;
+  float2 v;
+  for (; i + (kRun - 1) * step < end; sum.x += (double)v.x, sum.y += (double)v.y) {
+    v = per_both(0.f);
+#pragma unroll 8
+    for (int k = 0; k < kRun; ++k, i += step) f(i, v);
+  }
+  for (v = per_both(0.f); i < end; i += step) f(i, v);
+  sum.x += (double)v.x;
+  sum.y += (double)v.y;
+  return sum;
+}
+
 template <typename T, typename P>
-__global__ void __launch_bounds__(kThreads) per_layer_norm_long_kernel(const Fwd f) {
+__global__ void __launch_bounds__(kThreads, 6) per_layer_norm_long_kernel(const Fwd f) {
   per_wait_previous_grid();
-  const float n = (float)f.dim;
+  const double n = (double)f.dim;
   const P* w = static_cast<const P*>(f.w);
   const P* b = static_cast<const P*>(f.b);
   for (int64_t row = blockIdx.x; row < f.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(f.x) + row * f.x_stride;
     T* y = static_cast<T*>(f.y) + row * f.y_stride;
-    float a = 0.f, q = 0.f;
-    for (int64_t c = threadIdx.x; c < f.dim; c += kThreads) a += per_to_f32(x[c]);
-    const float s = block_sum2(a, 0.f).x / n;
-    a = 0.f;
-    for (int64_t c = threadIdx.x; c < f.dim; c += kThreads) {
+    const double2 all = long_sums(threadIdx.x, kThreads, f.dim,
+                                  [&](int64_t c, float2& v) { v.x += per_to_f32(x[c]); });
+    const float s = (float)(block_sum2(all.x, 0.0).x / n);
+    const double2 d = long_sums(threadIdx.x, kThreads, f.dim, [&](int64_t c, float2& v) {
       const float d = per_to_f32(x[c]) - s;
-      a += d;
-      q = fmaf(d, d, q);
-    }
-    const float2 t = block_sum2(a, q);
-    const float shift = t.x / n;
-    const float r = rsqrtf(fmaxf(t.y / n - shift * shift, 0.f) + f.eps);
+      v.x += d;
+      v.y = fmaf(d, d, v.y);
+    });
+    const double2 t = block_sum2(d.x, d.y);
+    const double off = t.x / n;
+    const float shift = (float)off;
+    const float r = rsqrtf((float)fmax(t.y / n - off * off, 0.0) + f.eps);
     for (int64_t c = threadIdx.x; c < f.dim; c += kThreads) {
       float h = (per_to_f32(x[c]) - s - shift) * r;
       if (w) h *= per_to_f32(w[c]);
@@ -1214,9 +1238,9 @@ __global__ void __launch_bounds__(kThreads) per_layer_norm_long_kernel(const Fwd
 }
 
 template <typename T, typename P>
-__global__ void __launch_bounds__(kThreads) per_layer_norm_dx_long_kernel(const Bwd g) {
+__global__ void __launch_bounds__(kThreads, 8) per_layer_norm_dx_long_kernel(const Bwd g) {
   per_wait_previous_grid();
-  const float n = (float)g.dim;
+  const double n = (double)g.dim;
   const P* w = static_cast<const P*>(g.w);
   for (int64_t row = blockIdx.x; row < g.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(g.x) + row * g.x_stride;
@@ -1224,15 +1248,14 @@ __global__ void __launch_bounds__(kThreads) per_layer_norm_dx_long_kernel(const 
     T* dx = static_cast<T*>(g.dx) + row * g.dx_stride;
     const float4 st = g.stats[row];
     const float hi = st.x, lo = st.y, r = st.z;
-    float a = 0.f, q = 0.f;
-    for (int64_t c = threadIdx.x; c < g.dim; c += kThreads) {
+    const double2 sums = long_sums(threadIdx.x, kThreads, g.dim, [&](int64_t c, float2& v) {
       const float h = (per_to_f32(x[c]) - hi - lo) * r;
       const float gv = per_to_f32(dy[c]) * (w ? per_to_f32(w[c]) : 1.f);
-      a += gv;
-      q = fmaf(gv, h, q);
-    }
-    const float2 t = block_sum2(a, q);
-    const float c1 = t.x / n, c2 = t.y / n;
+      v.x += gv;
+      v.y = fmaf(gv, h, v.y);
+    });
+    const double2 t = block_sum2(sums.x, sums.y);
+    const float c1 = (float)(t.x / n), c2 = (float)(t.y / n);
     for (int64_t c = threadIdx.x; c < g.dim; c += kThreads) {
       const float h = (per_to_f32(x[c]) - hi - lo) * r;
       const float gv = per_to_f32(dy[c]) * (w ? per_to_f32(w[c]) : 1.f);
@@ -1243,7 +1266,7 @@ __global__ void __launch_bounds__(kThreads) per_layer_norm_dx_long_kernel(const 
 
 // Column sums of one split of the rows: thread = column.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) per_layer_norm_dw_long_kernel(const Bwd g) {
+__global__ void __launch_bounds__(kThreads, 8) per_layer_norm_dw_long_kernel(const Bwd g) {
   per_wait_previous_grid();
   const int tiles = (g.dim - 1) / kThreads + 1;
   const int tile = blockIdx.x % tiles, split = blockIdx.x / tiles;
@@ -1251,16 +1274,14 @@ __global__ void __launch_bounds__(kThreads) per_layer_norm_dw_long_kernel(const 
   if (c >= g.dim) return;
   const T* x = static_cast<const T*>(g.x) + c;
   const T* dy = static_cast<const T*>(g.dy) + c;
-  float dw = 0.f, db = 0.f;
-  for (int64_t row = split; row < g.rows; row += g.splits) {
+  const double2 sums = long_sums(split, g.splits, g.rows, [&](int64_t row, float2& v) {
     const float4 st = g.stats[row];
-    const float hi = st.x, lo = st.y, r = st.z;
-    const float v = per_to_f32(dy[row * g.dy_stride]);
-    dw = fmaf(v, (per_to_f32(x[row * g.x_stride]) - hi - lo) * r, dw);
-    db += v;
-  }
-  g.part[(int64_t)split * 2 * g.places.padded + c] = dw;
-  g.part[((int64_t)split * 2 + 1) * g.places.padded + c] = db;
+    const float d = per_to_f32(dy[row * g.dy_stride]);
+    v.x = fmaf(d, (per_to_f32(x[row * g.x_stride]) - st.x - st.y) * st.z, v.x);
+    v.y += d;
+  });
+  g.part[(int64_t)split * 2 * g.places.padded + c] = (float)sums.x;
+  g.part[((int64_t)split * 2 + 1) * g.places.padded + c] = (float)sums.y;
 }
 
 // dw and db from the partial rows. A CTA adds 32 places: 8 threads take four
