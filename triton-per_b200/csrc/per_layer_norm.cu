@@ -1290,7 +1290,7 @@ __global__ void __launch_bounds__(kThreads, 8) per_layer_norm_dw_long_kernel(con
 constexpr int kJoinThreads = 512;
 template <typename P>
 __global__ void __launch_bounds__(kJoinThreads) per_layer_norm_join_kernel(const Bwd g) {
-  __shared__ float s[kJoinThreads / 32][32];
+  __shared__ __align__(16) float s[kJoinThreads / 32][32];  // stored by float4
   per_wait_previous_grid();
   const int quad = threadIdx.x & 7, team = threadIdx.x >> 3;
   const int64_t all = 2 * (int64_t)g.places.padded;
