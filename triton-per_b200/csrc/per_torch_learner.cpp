@@ -411,6 +411,7 @@ void clip_grads_with_norm(const py::list& params, double max_norm, const Tensor&
   const List l = list_of(params, true, "clip_grads_with_norm_");
   if (l.t.empty()) return;
   l.check_disjoint("clip_grads_with_norm_");
+  refuse_wrapped(norm, "clip_grads_with_norm_");
   if (norm.device() != l.device || norm.scalar_type() != at::kFloat || norm.numel() != 1)
     throw py::value_error("clip_grads_with_norm_: total_norm must be one float32 value on the "
                           "gradients' device");
@@ -419,8 +420,9 @@ void clip_grads_with_norm(const py::list& params, double max_norm, const Tensor&
         (uintptr_t)norm.data_ptr() < (uintptr_t)e.data + (uintptr_t)e.count * (e.dtype == PER_F32 ? 4 : 2))
       throw py::value_error("clip_grads_with_norm_: total_norm must not be part of a gradient");
   c10::cuda::CUDAGuard guard(l.device);
+  const Tensor value = plain(norm);
   check("per_scale_grads", per_scale_grads(l.t.data(), (int64_t)l.t.size(), (float)max_norm,
-                                           norm.data_ptr<float>(), l.stream()));
+                                           value.data_ptr<float>(), l.stream()));
   l.written();
 }
 
