@@ -48,10 +48,10 @@ def layer_norm_backward(dy, x, w, eps):
 
 
 def row_depth(dim: int) -> int:
-    """Additions in a row that a value's rounding error can pass through: at
-    most dim / 256 in one thread for the longest rows (up to 32 for the
-    others), the joins of a CTA, and the handful of operations around them."""
-    return 64 + dim // 256
+    """Additions in float32 that a row's value passes through: up to 32 in one
+    thread (longer rows join such sums in float64), the joins of a CTA or a
+    cluster, and the handful of operations around them."""
+    return 64
 
 
 def row_error(x, rstd):
@@ -89,7 +89,9 @@ def layer_norm_backward_bound(dy, x, w, eps, dtype, param_dtype):
     c2 = avg(g h) e avg(|g| (1 + 2 |h|)); dx = rstd (g - c1 - h c2) the sum of
     their shares plus the rounding of its own terms (each below e times its
     size). dw = sum dy h and db = sum dy pass through at most rows / 8 + 256
-    additions (the partial sums and their join) on top of the error of h."""
+    additions (the partial sums and their join) on top of the error of h. Over
+    many rows that bound exceeds the sums themselves; whole numbers that
+    float32 adds exactly show a lost row there."""
     _, mean, rstd = layer_norm(x, None, None, eps)
     h = ((x.double() - mean) * rstd)
     dx, dw, db = layer_norm_backward(dy, x, w, eps)
