@@ -17,10 +17,14 @@
 // operations a value, so that DRAM bounds every size beyond the L2 cache. What
 // a row costs beyond its values (the sums over its threads, addresses, waits)
 // decides how near a kernel comes, so rows are laid out by length (shape_of):
-//   - up to 512 or 1,024 values: LANES threads of a warp, several rows a warp;
-//   - up to 8,192 (backward) and 16,384 (forward) 16-bit values or 8,192
-//     float32 ones: a group of warps, rows copied ahead into shared memory;
-//   - up to eight times that: a cluster of CTAs, each with a slice;
+//   - up to 512 values, 16-bit ones up to 1,024 (512 in the backward pass of
+//     whole vectors): LANES threads of a warp, several rows a warp;
+//   - longer, whole vectors up to 8,192 values (16-bit forward: 16,384), rows that
+//     start anywhere up to half of that: a group of warps of one CTA, rows copied
+//     ahead into shared memory (forward, part of the upper half of whole vectors
+//     goes to clusters of two, see shape_of);
+//   - longer, up to 65,536 values (16-bit forward: 131,072): a cluster of up to 8
+//     CTAs, each with a slice;
 //   - longer: read from memory in each of two or three passes.
 // The columns' sums dw and db: a thread keeps those of its columns in registers
 // over all its rows; each CTA writes one partial row, and a second kernel adds
@@ -1346,12 +1350,13 @@ int sm_count() {
   return sms[dev];
 }
 
-// Row splits of the column sums of long rows.
+// Row splits of the column sums of long rows, for some 8 CTAs an SM: half of that
+// takes 1,765 us for 2000x131072 bfloat16 backward instead of 1,400; four times
+// as many take 0 to 11 % less, and as many times the partial rows.
 int splits_of(int64_t rows, int64_t dim) {
   const int64_t tiles = (dim - 1) / kThreads + 1;
   int64_t s = 1184 / tiles;
   if (s > rows) s = rows;
-  if (s > 256) s = 256;
   return s < 1 ? 1 : (int)s;
 }
 
@@ -1391,22 +1396,34 @@ Shape shape_of(int64_t dim, int vec, bool any, bool split, int singles, int full
   while (v > (int64_t)ctas * most_threads * full)
     if ((ctas *= 2) > kMaxCluster) return {0, 0, 0, 0};
   const auto threads = [&](int nv) { return (v + ctas * nv * 32 - 1) / (ctas * nv * 32) * 32; };
-  // An SM has registers for some 512 threads: CTAs of more than 256 leave some of
-  // them idle. Twice the CTAs then (20001 bfloat16 values, backward: 195 -> 162
-  // us; 10000 float32 ones, forward: 148 -> 122 us), except in the backward pass
-  // of whole vectors, where the wider cluster costs more (10000 float32 values:
-  // 153 -> 179 us).
+  // An SM has registers for some 512 threads: CTAs of more than 256 leave some
+  // of them idle. Twice the CTAs then. Forward, with and without, us: 16384x5000 float32 (320 threads) 114 and 136,
+  // 8192x10000 133 and 149, 8192x12288 bfloat16 (384) 79 and 90, but 16384x6000
+  // float32 (384) 158 and 150, 8192x12000 198 and 163; from 448 threads on the
+  // wider cluster costs more (8192x7600 float32 92 and 88, 4096x30000 266 and
+  // 206). Rows that start anywhere, both passes, up to a full CTA: 3000x20001
+  // bfloat16 backward 157 and 195, 8192x4201 float32 82 and 92, 106 and 119, but
+  // 8192x6001 114 and 100, 136 and 128. In the backward pass of whole vectors the
+  // wider cluster costs more (10000 float32 values: 153 -> 179 us).
   while (split && threads(full) > 256 && threads(full) < (any ? kRowThreads + 1 : 448) &&
          ctas < kMaxCluster)
     ctas *= 2;
-  // as many vectors a thread as there may be, or half, where that leaves fewer places empty
+  // As many vectors a thread as there may be, or half, where that leaves fewer
+  // places empty: rows of 513 to 768 values, or twice that in the forward pass of
+  // 16-bit ones. Few rows gain, us with half and with all: 512x768 float32 2.2
+  // and 2.4 forward, 256x768 4.1 and 5.1 backward, 512x1200 bfloat16 2.3 and 2.8
+  // forward. Of many, backward, 65536x768 float32 gains (95 and 102) and 65536x516
+  // loses (80 and 74); forward they lose (8192x768 14.3 and 11.3, 65536x768 98
+  // and 72).
   const int nv = threads(full / 2) <= most_threads && 8 * threads(full / 2) <= 13 * threads(full)
                      ? full / 2 : full;
   return {0, nv, (int)threads(nv), ctas};
 }
 
 // warp<T, P, VEC, NV, LANES>(...) or group<T, P, NV, CLUSTER, ANY>(...) for the
-// shape, into rc; false where there is none
+// shape, into rc; false where there is none. Half of F vectors a thread are for
+// rows of up to 48 F vectors: never a cluster's, and where rows start anywhere
+// only if these are more than a warp holds in single values.
 #define PER_NORM_SHAPE(s, rc, warp, group, T, P, ANY, FULL, ...)                               \
   [&]() -> bool {                                                                              \
     constexpr int V = ANY ? 1 : 16 / sizeof(T), S = ANY ? 4 : 1, F = FULL;                     \
@@ -1424,9 +1441,9 @@ Shape shape_of(int64_t dim, int vec, bool any, bool split, int singles, int full
       if (s.lanes == 32) return rc = warp<T, P, V, 8 * S, 32>(s, __VA_ARGS__), true;           \
     if (s.ctas == 1 && s.nv == F)                                                              \
       return rc = group<T, P, F, false, ANY>(s, __VA_ARGS__), true;                            \
-    if (s.ctas == 1) return rc = group<T, P, F / 2, false, ANY>(s, __VA_ARGS__), true;         \
-    if (s.ctas > 1 && s.nv == F) return rc = group<T, P, F, true, ANY>(s, __VA_ARGS__), true;  \
-    if (s.ctas > 1) return rc = group<T, P, F / 2, true, ANY>(s, __VA_ARGS__), true;           \
+    if constexpr (!ANY || 3 * F * 16 / (int)sizeof(T) > 2 * W)                                 \
+      if (s.ctas == 1) return rc = group<T, P, F / 2, false, ANY>(s, __VA_ARGS__), true;       \
+    if (s.ctas > 1) return rc = group<T, P, F, true, ANY>(s, __VA_ARGS__), true;               \
     return false;                                                                              \
   }()
 
@@ -1494,8 +1511,10 @@ int forward(const Fwd& f, cudaStream_t stream) {
   return forward_rows<T, P, true>(f, stream);
 }
 
-// Most partial rows of dw and db (the workspace is sized before the pointers'
-// alignment is known, so this holds for every kernel).
+// Most partial rows of dw and db: the workspace is sized before the pointers'
+// alignment, and with it the kernel, is known. No less than the CTAs that an SM
+// holds of any of them, so that it limits no grid (half and double of these
+// measure the same at nine sizes from 65536x32 to 4096x8192).
 int64_t most_partials(int64_t rows, int64_t dim) {
   const int64_t most = (int64_t)sm_count() * (dim <= 512 ? 8 : dim <= 2048 ? 4 : 2);
   return rows < most ? rows : most;
