@@ -342,7 +342,8 @@ typedef struct per_norm {
  * statistics for per_layer_norm_backward(): the mean as the sum of two floats
  * (a mean rounded to one float would cost (x - mean) * rstd as many units of
  * rounding as the mean is standard deviations), rstd, 0. NULL when no backward
- * pass follows. y must not overlap x. */
+ * pass follows. y must not overlap x. A row whose squared distances from the
+ * mean leave the float32 range has rstd 0: y = bias, and dx = 0. */
 int per_layer_norm(const per_norm_t* norm, const void* x, int64_t x_stride, const void* weight,
                    const void* bias, void* y, int64_t y_stride, float* stats, void* stream);
 

@@ -123,8 +123,9 @@ def _listed(tensors) -> list:
 
 def grad_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
     """The norm of all values of `tensors` (a tensor or an iterable of them,
-    of mixed types, on one device) as one vector: a float32 scalar on their
-    device, not differentiable. norm_type is 1, 2 or inf."""
+    of mixed types, on one device, each dense in its memory) as one vector: a
+    float32 scalar on their device, not differentiable. norm_type is 1, 2 or
+    inf."""
     kind = _kind(norm_type)
     norm = _binding().grad_norm(_listed(tensors), False, kind)
     return torch.tensor(0.0) if norm is None else norm
